@@ -14,6 +14,7 @@ LIB_PATH = os.path.join(_HERE, "lib", "libcfd_amd.so")
 F32, BF16 = 0, 1
 ACT_NONE, ACT_LEAKY, ACT_RELU, ACT_SIGMOID = 0, 1, 2, 3
 CONV_K4S2, CONV_K4S1, CONV_K3S1, CONVT_K4S2, DENSE, CONV_K4S1_BWD = 0, 1, 2, 3, 4, 5
+MX_X_F32, MX_X_BF16, MX_X_MXFP4 = 0, 1, 2
 TUNE_IGEMM256, TUNE_IGEMM256_PD, TUNE_WGRAD256, TUNE_CLASS_ORDER, TUNE_STAGED_OUT, TUNE_RESAMPLE_DENSITY, TUNE_NTILE, TUNE_PATCH = 0, 1, 2, 3, 4, 5, 6, 7
 TUNE_RESAMPLE_FUSED = 8
 TUNE_ONEPHASE = 9
@@ -25,6 +26,21 @@ class ConvDesc(C.Structure):
                 ("B", C.c_int), ("Hi", C.c_int), ("Wi", C.c_int), ("Cin", C.c_int), ("Cout", C.c_int),
                 ("ldx", C.c_int), ("ldy", C.c_int), ("act", C.c_int), ("leaky_slope", C.c_float),
                 ("split_k", C.c_int)]
+
+
+class AdamwTensor(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("g", C.c_void_p), ("copy", C.c_void_p), ("n", C.c_int64), ("state_offset", C.c_int64),
+                ("weight_decay", C.c_float)]
+
+
+class AdamwDesc(C.Structure):
+    _fields_ = [("p_dtype", C.c_int), ("g_dtype", C.c_int), ("state_bits", C.c_int), ("seed", C.c_uint),
+                ("lr", C.c_float), ("eps", C.c_float), ("beta1", C.c_double), ("beta2", C.c_double)]
+
+
+class Mxfp4DenseDesc(C.Structure):
+    _fields_ = [("x_kind", C.c_int), ("out_dtype", C.c_int), ("act", C.c_int), ("leaky_slope", C.c_float),
+                ("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64), ("ldx", C.c_int64), ("ldy", C.c_int64)]
 
 
 class CfdError(RuntimeError):
@@ -84,6 +100,14 @@ SIGNATURES = {
     "cfd_field_loss": (_i, [_vp, _vp, _i64, _i, _f, _f, _vp, _vp, _vp, _i, _vp]),
     "cfd_mfma_probe": (_i, [_vp, _vp, _i, _vp]),
     "cfd_adam_step": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i64, _f, _f, _f, _f, _f, _vp]),
+    "cfd_grad_norm_workspace_bytes": (_i64, [_vp, _i]),
+    "cfd_grad_norm": (_i, [_vp, _vp, _i, _i, _f, _vp, _vp, _vp]),
+    "cfd_adamw_step": (_i, [_vp, _i, C.POINTER(AdamwDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "cfd_mxfp4_scale_pitch": (_i64, [_i64]),
+    "cfd_mxfp4_quantize": (_i, [_vp, _i64, _i, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "cfd_mxfp4_dequantize": (_i, [_vp, _vp, _i64, _i64, _vp, _i64, _i, _vp]),
+    "cfd_mxfp4_dense_workspace_bytes": (_i64, [_i64, _i64, _i64, _i]),
+    "cfd_mxfp4_dense": (_i, [C.POINTER(Mxfp4DenseDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "cfd_bn_update_moving": (_i, [_vp, _vp, _vp, _vp, _i, _i, _f, _vp]),
     "cfd_bn_update_moving_multi": (_i, [_i, _vp, _vp, _vp, _vp, _vp, _i, _f, _vp]),
     "cfd_zero_ranges": (_i, [_vp, _vp, _i, _i64, _vp]),

@@ -22,6 +22,7 @@ ARCH = "gfx950"
 EXTRA = {
     "resample.hip": ["-ffp-contract=off"],   # bit-exact fp64: no fused multiply-add
     "dataset.hip": ["-ffp-contract=off"],
+    "optim.hip": ["-ffp-contract=off"],      # the 8-bit state's codes follow from single fp32 roundings
 }
 COMMON = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-function",
           "-Wno-unused-variable", "-fno-gpu-rdc",

@@ -1,0 +1,508 @@
+// 4-bit microscaled storage (OCP MX: E2M1 codes, one E8M0 power of two for 32 of them) and the Dense layer on it.
+//
+// A matrix of R rows x K columns, blocked along K: codes [R][16 nb] bytes (nb = ceil(K / 32); the low nibble is the lower
+// column), scales [R][16 ceil(nb / 16)] bytes.  Codes past K are zero, scale bytes past nb are 0 (2^-127 x 0): a
+// contraction may run over whole blocks and whole 512-column groups without masks.
+//
+// Quantisation: e = floor(log2 max|x|) - 2, one more where max|x| > 7 * 2^e, so that no element is off by more than half
+// a spacing at its block's top (the plain floor would clip a block's largest values by up to a quarter); codes round to
+// nearest even.  A block with an infinity or NaN gets the scale 0xFF: the whole block reads as NaN.
+#include "common.h"
+
+namespace cfd {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef __bf16 bf16x8a2 __attribute__((ext_vector_type(8), aligned(2)));
+typedef __bf16 bf16x4a2 __attribute__((ext_vector_type(4), aligned(2)));
+
+static inline int64_t mx_blocks(int64_t k) { return (k + 31) / 32; }
+static inline int64_t mx_scale_pitch(int64_t k) { return (mx_blocks(k) + 15) / 16 * 16; }
+
+// eight consecutive values at element alignment; `left` of them exist, the rest read as zero
+__device__ __forceinline__ void load8(const float *p, int left, float (&o)[8]) {
+  if (left >= 8) {
+    const f32x4a4 a = *(const f32x4a4 *)p, b = *(const f32x4a4 *)(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { o[i] = a[i]; o[4 + i] = b[i]; }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = i < left ? p[i] : 0.f;
+  }
+}
+__device__ __forceinline__ void load8(const bf16 *p, int left, float (&o)[8]) {
+  if (left >= 8) {
+    const bf16x8a2 a = *(const bf16x8a2 *)p;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = (float)a[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) o[i] = i < left ? (float)p[i] : 0.f;
+  }
+}
+
+// E8M0 byte of a block whose largest magnitude has these bits (NaN compares largest)
+__device__ __forceinline__ unsigned mx_scale_byte(unsigned amax) {
+  if (amax >= 0x7f800000u) return 255u;
+  const int f = (int)((amax + 0x1fffffu) >> 23) - 2;   // mantissa over 1.75 carries into the exponent
+  return f < 0 ? 0u : (unsigned)f;
+}
+// the hardware conversions take the scale as an fp32 power of two; a byte of 0 is the subnormal 2^-127
+__device__ __forceinline__ float mx_scale_f32(unsigned byte) {
+  return __uint_as_float(byte ? byte << 23 : 0x00400000u);
+}
+__device__ __forceinline__ unsigned mx_code8(const float (&x)[8], unsigned byte) {
+  const float s = mx_scale_f32(byte);
+  unsigned c = 0;
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[0], x[1], s, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[2], x[3], s, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[4], x[5], s, 2);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[6], x[7], s, 3);
+  return byte == 255u ? 0u : c;
+}
+__device__ __forceinline__ unsigned amax8(const float (&x)[8]) {
+  unsigned a = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a = max(a, __float_as_uint(x[i]) & 0x7fffffffu);
+  return a;
+}
+__device__ __forceinline__ unsigned quad_umax(unsigned v) {
+  v = max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false));   // lane ^ 1
+  return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));  // lane ^ 2
+}
+
+// scale byte of block b, and the zero bytes behind the last block
+__device__ __forceinline__ void put_scale(uint8_t *row, int b, int nb, int pitch, unsigned byte) {
+  row[b] = (uint8_t)byte;
+  if (b == nb - 1)
+    for (int i = nb; i < pitch; ++i) row[i] = 0;
+}
+
+// rows only: four lanes share a block of 32 (eight columns each): 32-byte / 16-byte loads, 4-byte stores, the block's
+// maximum in two DPP steps.  HBM-bound: s_in + 0.53 bytes an element.
+template <typename T> __global__ __launch_bounds__(256) void mx_quant_rows_kernel(const T *x, int64_t ldx, int64_t rows, int K,
+                                                                                   int nb, int pitch, uint8_t *codes,
+                                                                                   uint8_t *scales) {
+  const int64_t G = (int64_t)nb * 4, total = rows * G;
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= total) return;                 // (whole quads: G is a multiple of 4)
+  const int64_t row = t / G;
+  const int grp = (int)(t - row * G);
+  float v[8];
+  load8(x + row * ldx + (int64_t)grp * 8, K - grp * 8, v);
+  const unsigned byte = mx_scale_byte(quad_umax(amax8(v)));
+  *(unsigned *)(codes + row * nb * 16 + (int64_t)grp * 4) = mx_code8(v, byte);
+  if ((grp & 3) == 0) put_scale(scales + row * pitch, grp >> 2, nb, pitch, byte);
+}
+
+// both orientations from one read: a 128 x 64 tile; rows are coded on the way in, columns from LDS.  The tile's columns
+// are swizzled by 16 per 32 rows so that the four row blocks a quad of lanes reads fall into different banks.
+constexpr int QT_R = 128, QT_C = 64;
+template <typename T> __global__ __launch_bounds__(256) void mx_quant_both_kernel(const T *x, int64_t ldx, int R, int K,
+                                                                                   int nb, int pitch, uint8_t *codes,
+                                                                                   uint8_t *scales, int nbt, int pitch_t,
+                                                                                   uint8_t *codes_t, uint8_t *scales_t) {
+  __shared__ float tile[QT_R * QT_C];
+  const int r0 = blockIdx.y * QT_R, c0 = blockIdx.x * QT_C;
+  const int tid = threadIdx.x;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int r = i * 32 + (tid >> 3), c = (tid & 7) * 8;
+    float v[8];
+    load8(x + (int64_t)(r0 + r) * ldx + c0 + c, r0 + r < R ? K - c0 - c : 0, v);
+    float *dst = tile + r * QT_C + (c ^ ((r >> 5) * 16));
+    *(f32x4 *)dst = (f32x4){v[0], v[1], v[2], v[3]};
+    *(f32x4 *)(dst + 4) = (f32x4){v[4], v[5], v[6], v[7]};
+    if (codes) {
+      const unsigned byte = mx_scale_byte(quad_umax(amax8(v)));
+      const int b = (c0 + c) >> 5;
+      if (r0 + r < R && b < nb) {
+        *(unsigned *)(codes + (int64_t)(r0 + r) * nb * 16 + (c0 + c) / 2) = mx_code8(v, byte);
+        if ((tid & 3) == 0) put_scale(scales + (int64_t)(r0 + r) * pitch, b, nb, pitch, byte);
+      }
+    }
+  }
+  __syncthreads();
+  const int c = tid >> 2, rb = tid & 3;      // one column's 32 rows
+  const int bt = (r0 >> 5) + rb;
+  if (c0 + c >= K || bt >= nbt) return;
+  float v[4][8];
+  unsigned am = 0;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[g][i] = tile[(rb * 32 + g * 8 + i) * QT_C + (c ^ (rb * 16))];
+    am = max(am, amax8(v[g]));
+  }
+  const unsigned byte = mx_scale_byte(am);
+  i32x4 o;
+#pragma unroll
+  for (int g = 0; g < 4; ++g) o[g] = (int)mx_code8(v[g], byte);
+  *(i32x4 *)(codes_t + (int64_t)(c0 + c) * nbt * 16 + bt * 16) = o;
+  put_scale(scales_t + (int64_t)(c0 + c) * pitch_t, bt, nbt, pitch_t, byte);
+}
+
+// codes -> values: a lane reads eight codes and writes 16 (bf16) or 32 (fp32) bytes
+template <typename T> __global__ __launch_bounds__(256) void mx_dequant_kernel(const uint8_t *codes, const uint8_t *scales,
+                                                                                int64_t rows, int K, int nb, int pitch, T *y,
+                                                                                int64_t ldy) {
+  const int64_t G = (int64_t)nb * 4, total = rows * G;
+  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (t >= total) return;
+  const int64_t row = t / G;
+  const int grp = (int)(t - row * G), left = K - grp * 8;
+  const unsigned c = *(const unsigned *)(codes + row * nb * 16 + (int64_t)grp * 4);
+  const unsigned byte = scales[row * pitch + (grp >> 2)];
+  const float s = byte == 255u ? __uint_as_float(0x7fc00000u) : mx_scale_f32(byte);
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f32x2 p = i == 0   ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 0)
+                    : i == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 1)
+                    : i == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 2)
+                             : __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 3);
+    v[2 * i] = p[0] * s;          // exact, or an overflow to infinity at the top of the scale's range
+    v[2 * i + 1] = p[1] * s;
+  }
+  T *o = y + row * ldy + (int64_t)grp * 8;
+  if (left >= 8) {
+    if constexpr (sizeof(T) == 2) {
+      bf16x8a2 w;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) w[i] = (bf16)v[i];
+      *(bf16x8a2 *)o = w;
+    } else {
+      *(f32x4a4 *)o = (f32x4){v[0], v[1], v[2], v[3]};
+      *(f32x4a4 *)(o + 4) = (f32x4){v[4], v[5], v[6], v[7]};
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < left) o[i] = (T)v[i];
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------- products
+struct MxDense {
+  const uint8_t *xc, *xs, *wc, *ws;   // 4-bit operands: activations (M rows), weights (N rows)
+  const void *x;                      // or float activations
+  int64_t ldx;
+  const float *bias;
+  void *y;
+  int64_t ldy;
+  float *slab;                        // [split][M][N] partial sums (split > 1)
+  int M, N, K, nb, pitch;
+  int split, kt_per;                  // K groups (256 or 512 columns) per split
+  int mt, nt;
+  int out_bf16, act;
+  float slope;
+};
+
+__device__ __forceinline__ void mx_store(const MxDense &p, int64_t m, int n, float v) {   // one element of the output
+  if (p.out_bf16) ((bf16 *)p.y)[m * p.ldy + n] = (bf16)v;
+  else ((float *)p.y)[m * p.ldy + n] = v;
+}
+// lane's four consecutive outputs n..n+3 of row m
+__device__ __forceinline__ void mx_emit(const MxDense &p, int sk, int64_t m, int n, f32x4 v) {
+  if (m >= p.M || n >= p.N) return;
+  if (p.split > 1) {
+    float *o = p.slab + ((int64_t)sk * p.M + m) * p.N + n;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (n + r < p.N) o[r] = v[r];
+    return;
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (n + r < p.N) mx_store(p, m, n + r, apply_act(v[r] + (p.bias ? p.bias[n + r] : 0.f), p.act, p.slope));
+}
+
+// sums of the split slabs in a fixed order, bias, activation, output type
+__global__ __launch_bounds__(256) void mx_split_sum_kernel(MxDense p) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, MN = (int64_t)p.M * p.N;
+  if (i >= MN) return;
+  float s = 0.f;
+  for (int k = 0; k < p.split; ++k) s += p.slab[k * MN + i];
+  const int64_t m = i / p.N;
+  const int n = (int)(i - m * p.N);
+  mx_store(p, m, n, apply_act(s + (p.bias ? p.bias[n] : 0.f), p.act, p.slope));
+}
+
+constexpr unsigned MX_OOB = 0x80000000u;
+__device__ __forceinline__ i32x4 ld16(__amdgpu_buffer_rsrc_t r, unsigned off) {
+  return __builtin_amdgcn_raw_buffer_load_b128(r, (int)off, 0, 0);
+}
+__device__ __forceinline__ i32x8 wide(i32x4 a) { return (i32x8){a[0], a[1], a[2], a[3], 0, 0, 0, 0}; }
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_rsrc(const uint8_t *base, int64_t row0, int rows, int64_t pitch) {
+  // tile-relative: rows past the operand fall out of range and read as zero, and no offset needs more than 31 bits
+  return __builtin_amdgcn_make_buffer_rsrc((void *)(base + row0 * pitch), 0, (int)(rows * pitch), 0x00020000);
+}
+
+// Both operands in 4 bits, any shape: a workgroup of four waves owns 64 (m) x 64 (n), a wave 32 x 32, fragments go from
+// global memory straight into the scaled MFMA (16x16x128: lane = row l & 15, block l >> 4; its scale byte is the lane's own).
+// A K group is 256 columns = two MFMA steps; lane group g takes the blocks 2g and 2g + 1 of the group, so one 16-bit load
+// holds both of its scales and the step picks the byte.
+__global__ __launch_bounds__(256) void mx_dense_kernel(MxDense p) {
+  int bid = blockIdx.x;
+  const int nt = bid % p.nt; bid /= p.nt;
+  const int mt = bid % p.mt;
+  const int sk = bid / p.mt;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
+  const int m0 = mt * 64, n0 = nt * 64;
+  const int cp = p.nb * 16;
+  const int mr = min(64, p.M - m0), nr = min(64, p.N - n0);
+  const __amdgpu_buffer_rsrc_t xr = mx_rsrc(p.xc, m0, mr, cp), wr = mx_rsrc(p.wc, n0, nr, cp);
+  const __amdgpu_buffer_rsrc_t xsr = mx_rsrc(p.xs, m0, mr, p.pitch), wsr = mx_rsrc(p.ws, n0, nr, p.pitch);
+  const int wm = (wave & 1) * 32, wn = (wave >> 1) * 32;
+  f32x4 acc[2][2] = {};
+  const int k0 = sk * p.kt_per, k1 = min(k0 + p.kt_per, (p.nb + 7) / 8);
+  for (int kt = k0; kt < k1; ++kt) {
+    const int b0 = kt * 8 + fq * 2;
+    i32x4 a[2][2], b[2][2];
+    int as[2], bs[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int rw = wn + i * 16 + fr, rx = wm + i * 16 + fr;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        a[i][s] = ld16(wr, b0 + s < p.nb && rw < nr ? (unsigned)(rw * cp + (b0 + s) * 16) : MX_OOB);
+        b[i][s] = ld16(xr, b0 + s < p.nb && rx < mr ? (unsigned)(rx * cp + (b0 + s) * 16) : MX_OOB);
+      }
+      as[i] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(wsr, rw < nr ? (int)(rw * p.pitch + b0) : (int)MX_OOB, 0, 0);
+      bs[i] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(xsr, rx < mr ? (int)(rx * p.pitch + b0) : (int)MX_OOB, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(a[i][0]), wide(b[j][0]), acc[i][j], 4, 4, 0, as[i], 0, bs[j]);
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(a[i][1]), wide(b[j][1]), acc[i][j], 4, 4, 1, as[i], 1, bs[j]);
+      }
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) mx_emit(p, sk, m0 + wm + j * 16 + fr, n0 + wn + i * 16 + fq * 4, acc[i][j]);
+}
+
+// Float activations against 4-bit weights (serving: the weights are what is read).  A wave owns 64 weight rows x 16
+// activation rows; a K group is 512 columns: lane group g takes blocks 4g..4g+3, so a lane reads 64 contiguous bytes of
+// codes and one 32-bit word of scales.  Codes become bf16 with their scale applied (exact: two significant bits) and meet
+// the activations in 16x16x32 bf16 MFMAs, whose k order is the lane's block order on both operands.  fp32 activations are
+// split exactly into three bf16 terms (8 + 8 + 8 bits by truncation) and take three MFMAs: fp32 accuracy, the weights
+// are still read once.  The four waves of a workgroup take K groups in turn and join in LDS.
+struct Split3 { bf16 t[3]; };
+__device__ __forceinline__ Split3 split3(float x) {
+  Split3 r;
+  const unsigned u = __float_as_uint(x);
+  if ((u & 0x7f800000u) == 0x7f800000u) {          // infinity, NaN: one term carries it
+    r.t[0] = (bf16)x; r.t[1] = (bf16)0.f; r.t[2] = (bf16)0.f;
+    return r;
+  }
+  const float h = __uint_as_float(u & 0xffff0000u), d = x - h;
+  const float m = __uint_as_float(__float_as_uint(d) & 0xffff0000u);
+  r.t[0] = (bf16)h; r.t[1] = (bf16)m; r.t[2] = (bf16)(d - m);
+  return r;
+}
+__device__ __forceinline__ bf16x8 mx_bf16x8(unsigned c, float s) {
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2), e = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3);
+  return (bf16x8){a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1]};
+}
+
+template <typename TX> __global__ __launch_bounds__(256) void mx_serve_kernel(MxDense p) {
+  constexpr int NX = sizeof(TX) == 4 ? 3 : 1;
+  __shared__ f32x4 part[4][4][64];
+  int bid = blockIdx.x;
+  const int nt = bid % p.nt; bid /= p.nt;
+  const int mt = bid % p.mt;
+  const int sk = bid / p.mt;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
+  const int m = mt * 16 + fr, n0 = nt * 64;
+  const int cp = p.nb * 16, nr = min(64, p.N - n0);
+  const __amdgpu_buffer_rsrc_t wr = mx_rsrc(p.wc, n0, nr, cp), wsr = mx_rsrc(p.ws, n0, nr, p.pitch);
+  const TX *x = (const TX *)p.x + (int64_t)m * p.ldx;
+  f32x4 acc[4] = {};
+  const int k0 = sk * p.kt_per, k1 = min(k0 + p.kt_per, (p.nb + 15) / 16);
+  for (int kt = k0 + wave; kt < k1; kt += 4) {
+    const int b0 = kt * 16 + fq * 4;
+    i32x4 c[4][4];
+    unsigned sc[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = i * 16 + fr;
+      sc[i] = (unsigned)__builtin_amdgcn_raw_buffer_load_b32(wsr, r < nr ? (int)(r * p.pitch + b0) : (int)MX_OOB, 0, 0);
+#pragma unroll
+      for (int s = 0; s < 4; ++s) c[i][s] = ld16(wr, b0 + s < p.nb && r < nr ? (unsigned)(r * cp + (b0 + s) * 16) : MX_OOB);
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      float sf[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned byte = (sc[i] >> (8 * s)) & 255u;
+        sf[i] = byte == 255u ? __uint_as_float(0x7fc00000u) : mx_scale_f32(byte);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int k = (b0 + s) * 32 + j * 8;
+        float v[8];
+        if (m < p.M && k < p.K) load8(x + k, p.K - k, v);
+        else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = 0.f;
+        }
+        bf16x8 xb[NX];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if constexpr (NX == 1) xb[0][e] = (bf16)v[e];
+          else {
+            const Split3 q = split3(v[e]);
+#pragma unroll
+            for (int t = 0; t < 3; ++t) xb[t][e] = q.t[t];
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bf16x8 wv = mx_bf16x8((unsigned)c[i][s][j], sf[i]);
+#pragma unroll
+          for (int t = NX - 1; t >= 0; --t) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xb[t], acc[i], 0, 0, 0);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) part[wave][i][lane] = acc[i];
+  __syncthreads();
+  f32x4 t = part[0][wave][lane];
+#pragma unroll
+  for (int w = 1; w < 4; ++w) t += part[w][wave][lane];
+  mx_emit(p, sk, m, n0 + wave * 16 + fq * 4, t);
+}
+
+static int mx_check(int64_t m, int64_t n, int64_t k) {
+  CFD_REQUIRE(m >= 0 && n >= 0 && m <= 0x7fffff00 && n <= 0x7fffff00, "rows out of range");
+  CFD_REQUIRE(k > 0 && k <= (1 << 22), "columns must be in 1 .. 4194304");
+  return CFD_OK;
+}
+
+// K slices: enough workgroups to fill the chip (4 per CU), no slice under `least` groups
+static void mx_split(MxDense &p, int groups, int64_t tiles, int least) {
+  int64_t want = 1024 / tiles;
+  if (want > groups / least) want = groups / least;
+  if (want < 1) want = 1;
+  p.kt_per = (int)((groups + want - 1) / want);
+  p.split = (groups + p.kt_per - 1) / p.kt_per;
+}
+static void mx_plan(MxDense &p, bool serve) {
+  p.nb = (int)mx_blocks(p.K);
+  p.pitch = (int)mx_scale_pitch(p.K);
+  p.nt = (p.N + 63) / 64;
+  p.mt = serve ? (p.M + 15) / 16 : (p.M + 63) / 64;
+  mx_split(p, serve ? (p.nb + 15) / 16 : (p.nb + 7) / 8, (int64_t)p.nt * p.mt, 4);
+}
+
+}  // namespace cfd
+
+using namespace cfd;
+
+extern "C" int64_t cfd_mxfp4_scale_pitch(int64_t cols) { return mx_scale_pitch(cols); }
+
+extern "C" int cfd_mxfp4_quantize(const void *x, int64_t ldx, int dtype, int64_t rows, int64_t cols, uint8_t *codes,
+                                  uint8_t *scales, uint8_t *codes_t, uint8_t *scales_t, void *stream) {
+  if (int rc = mx_check(rows, 0, cols)) return rc;
+  CFD_REQUIRE(dtype == CFD_F32 || dtype == CFD_BF16, "bad dtype");
+  if (rows == 0) return CFD_OK;
+  CFD_REQUIRE((codes != nullptr) == (scales != nullptr) && (codes_t != nullptr) == (scales_t != nullptr) && (codes || codes_t),
+              "codes come with scales, in one orientation at least");
+  CFD_REQUIRE(x && ldx >= cols, "bad arguments");
+  CFD_REQUIRE(((uintptr_t)codes & 15) == 0 && ((uintptr_t)codes_t & 15) == 0, "codes must be 16-byte aligned");
+  hipStream_t st = (hipStream_t)stream;
+  const int nb = (int)mx_blocks(cols), pitch = (int)mx_scale_pitch(cols);
+  if (!codes_t) {
+    const int64_t blocks = (rows * nb * 4 + 255) / 256;
+    CFD_REQUIRE(blocks <= 0x7fffffff, "too many elements");
+    if (dtype == CFD_BF16)
+      hipLaunchKernelGGL(mx_quant_rows_kernel<bf16>, dim3((unsigned)blocks), dim3(256), 0, st, (const bf16 *)x, ldx, rows,
+                         (int)cols, nb, pitch, codes, scales);
+    else
+      hipLaunchKernelGGL(mx_quant_rows_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, st, (const float *)x, ldx, rows,
+                         (int)cols, nb, pitch, codes, scales);
+  } else {
+    if (int rc = mx_check(cols, 0, rows)) return rc;   // the rows are the other orientation's columns
+    const int nbt = (int)mx_blocks(rows), pitch_t = (int)mx_scale_pitch(rows);
+    const dim3 grid((unsigned)((cols + QT_C - 1) / QT_C), (unsigned)((rows + QT_R - 1) / QT_R));
+    if (dtype == CFD_BF16)
+      hipLaunchKernelGGL(mx_quant_both_kernel<bf16>, grid, dim3(256), 0, st, (const bf16 *)x, ldx, (int)rows, (int)cols, nb,
+                         pitch, codes, scales, nbt, pitch_t, codes_t, scales_t);
+    else
+      hipLaunchKernelGGL(mx_quant_both_kernel<float>, grid, dim3(256), 0, st, (const float *)x, ldx, (int)rows, (int)cols, nb,
+                         pitch, codes, scales, nbt, pitch_t, codes_t, scales_t);
+  }
+  CFD_LAUNCH_CHECK();
+  return CFD_OK;
+}
+
+extern "C" int cfd_mxfp4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t cols, void *y, int64_t ldy,
+                                    int dtype, void *stream) {
+  if (int rc = mx_check(rows, 0, cols)) return rc;
+  CFD_REQUIRE(dtype == CFD_F32 || dtype == CFD_BF16, "bad dtype");
+  if (rows == 0) return CFD_OK;
+  CFD_REQUIRE(codes && scales && y && ldy >= cols, "bad arguments");
+  const int nb = (int)mx_blocks(cols), pitch = (int)mx_scale_pitch(cols);
+  const int64_t blocks = (rows * nb * 4 + 255) / 256;
+  CFD_REQUIRE(blocks <= 0x7fffffff, "too many elements");
+  if (dtype == CFD_BF16)
+    hipLaunchKernelGGL(mx_dequant_kernel<bf16>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, codes, scales, rows,
+                       (int)cols, nb, pitch, (bf16 *)y, ldy);
+  else
+    hipLaunchKernelGGL(mx_dequant_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, codes, scales, rows,
+                       (int)cols, nb, pitch, (float *)y, ldy);
+  CFD_LAUNCH_CHECK();
+  return CFD_OK;
+}
+
+extern "C" int64_t cfd_mxfp4_dense_workspace_bytes(int64_t m, int64_t n, int64_t k, int x_float) {
+  if (int rc = mx_check(m, n, k)) return rc;
+  if (!m || !n) return 0;
+  MxDense p = {};
+  p.M = (int)m; p.N = (int)n; p.K = (int)k;
+  mx_plan(p, x_float != 0);
+  return p.split > 1 ? (int64_t)p.split * m * n * 4 : 0;
+}
+
+extern "C" int cfd_mxfp4_dense(const cfd_mxfp4_dense_desc *d, const void *x, const uint8_t *x_scales, const uint8_t *w_codes,
+                               const uint8_t *w_scales, const float *bias, void *y, void *ws, void *stream) {
+  CFD_REQUIRE(d, "NULL descriptor");
+  if (int rc = mx_check(d->m, d->n, d->k)) return rc;
+  CFD_REQUIRE(d->x_kind == CFD_MX_X_MXFP4 || d->x_kind == CFD_MX_X_F32 || d->x_kind == CFD_MX_X_BF16, "bad x_kind");
+  CFD_REQUIRE(d->out_dtype == CFD_F32 || d->out_dtype == CFD_BF16, "bad out_dtype");
+  CFD_REQUIRE(d->act >= CFD_ACT_NONE && d->act <= CFD_ACT_SIGMOID, "bad activation");
+  if (!d->m || !d->n) return CFD_OK;
+  const bool serve = d->x_kind != CFD_MX_X_MXFP4;
+  CFD_REQUIRE(x && w_codes && w_scales && y && d->ldy >= d->n, "bad arguments");
+  CFD_REQUIRE(serve ? d->ldx >= d->k : x_scales != nullptr, "bad activations");
+  CFD_REQUIRE((((uintptr_t)w_codes | (uintptr_t)w_scales) & 15) == 0, "weights must be 16-byte aligned");
+  CFD_REQUIRE(serve || (((uintptr_t)x | (uintptr_t)x_scales) & 15) == 0, "4-bit activations must be 16-byte aligned");
+  MxDense p = {};
+  p.M = (int)d->m; p.N = (int)d->n; p.K = (int)d->k;
+  mx_plan(p, serve);
+  p.xc = (const uint8_t *)x; p.xs = x_scales; p.x = x; p.ldx = d->ldx; p.wc = w_codes; p.ws = w_scales; p.bias = bias;
+  p.y = y; p.ldy = d->ldy; p.out_bf16 = d->out_dtype == CFD_BF16; p.act = d->act; p.slope = d->leaky_slope;
+  p.slab = (float *)ws;
+  CFD_REQUIRE(p.split == 1 || ws, "this shape needs a workspace");
+  const int64_t blocks = (int64_t)p.mt * p.nt * p.split;
+  CFD_REQUIRE(blocks <= 0x7fffffff, "too many tiles");
+  hipStream_t st = (hipStream_t)stream;
+  if (d->x_kind == CFD_MX_X_MXFP4) hipLaunchKernelGGL(mx_dense_kernel, dim3((unsigned)blocks), dim3(256), 0, st, p);
+  else if (d->x_kind == CFD_MX_X_BF16) hipLaunchKernelGGL(mx_serve_kernel<bf16>, dim3((unsigned)blocks), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL(mx_serve_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, st, p);
+  CFD_LAUNCH_CHECK();
+  if (p.split > 1) {
+    const int64_t b = (d->m * d->n + 255) / 256;
+    hipLaunchKernelGGL(mx_split_sum_kernel, dim3((unsigned)b), dim3(256), 0, st, p);
+    CFD_LAUNCH_CHECK();
+  }
+  return CFD_OK;
+}

@@ -6,15 +6,16 @@ buffer (that is how concat buffers are written in place); `_nhwc` turns it into 
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import numpy as np
 import torch
 
 from . import _lib
 from ._lib import (ACT_LEAKY, ACT_NONE, ACT_RELU, ACT_SIGMOID, BF16, CONV_K3S1, CONV_K4S1, CONV_K4S2, CONVT_K4S2,
-                   DENSE, F32, TUNE_CLASS_ORDER, TUNE_IGEMM256, TUNE_STAGED_OUT, TUNE_IGEMM256_PD, TUNE_WGRAD256, TUNE_NTILE, TUNE_PATCH, TUNE_RESAMPLE_FUSED, TUNE_ONEPHASE, TUNE_SKINNY, ConvDesc, check)
+                   DENSE, F32, TUNE_CLASS_ORDER, TUNE_IGEMM256, TUNE_STAGED_OUT, TUNE_IGEMM256_PD, TUNE_WGRAD256, TUNE_NTILE, TUNE_PATCH, TUNE_RESAMPLE_FUSED, TUNE_ONEPHASE, TUNE_SKINNY, AdamwDesc, AdamwTensor, ConvDesc, Mxfp4DenseDesc, check)
 
 LEAKY_SLOPE = 0.2
 _DT = {torch.float32: F32, torch.bfloat16: BF16}
@@ -912,3 +913,201 @@ def conv_first_wgrad(x, x2, dpre, dw, db, ksize, stride):
     check(_lib.load().cfd_conv_first_wgrad(_ptr(x), _ptr(x2), c1, c2, dp, ldd, _ptr(dw), _ptr(db), B, Hi, Wi,
                                            dpre.shape[-1], ksize, stride, _DT[dpre.dtype], _stream()),
           "cfd_conv_first_wgrad")
+
+
+# ----------------------------------------------------------------------------------------
+# optimizer over a list of tensors (trainer.AdamW keeps the state)
+# ----------------------------------------------------------------------------------------
+def _on(device: torch.device):
+    """launches go to the tensors' device and its current stream, whatever device is current"""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _tensor_list(ts: Sequence[torch.Tensor], what: str, dtype: Optional[torch.dtype] = None,
+                 device: Optional[torch.device] = None) -> None:
+    """dense device tensors of one dtype (fp32 or bf16) on one device"""
+    for t in ts:
+        dtype, device = dtype or t.dtype, device or t.device
+        if not t.is_cuda or t.dtype != dtype or t.device != device or not t.is_contiguous():
+            _dev(t)
+            _need(t.device == device, f"{what} on {t.device}, the others on {device}")
+            _need(t.dtype == dtype, f"{what} must share one dtype, {dtype} and {t.dtype} given")
+            _need(False, f"{what} must be contiguous, shape {tuple(t.shape)} strides {tuple(t.stride())}")
+    _need(dtype in _DT or dtype is None, f"{what} must be fp32 or bf16, is {dtype}")
+
+
+def grad_norm(grads: Union[torch.Tensor, Sequence[torch.Tensor]], max_norm: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """fp32 device tensor [norm, scale]: the L2 norm over all elements of `grads` (dense tensors of one dtype, any length) and
+    min(1, max_norm / norm), NaN where the norm is not finite.  Nothing waits for the device: hand out[1:] to
+    trainer.AdamW.step as `grad_scale` and the step is clipped, or skipped on a non-finite gradient."""
+    lib = _lib.load()
+    grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+    _need(len(grads) > 0, "grad_norm needs at least one tensor")
+    _need(max_norm > 0, f"grad_norm: max_norm must be positive, is {max_norm}")
+    _tensor_list(grads, "grad_norm: gradients")
+    n = len(grads)
+    ptrs = (C.c_void_p * n)(*[g.data_ptr() for g in grads])
+    sizes = (C.c_int64 * n)(*[g.numel() for g in grads])
+    dev = grads[0].device
+    with _on(dev):
+        if out is None:
+            out = torch.empty(2, dtype=torch.float32, device=dev)
+        _numel(out, 2, "grad_norm out", torch.float32)
+        _need(out.device == dev, "grad_norm: out must be on the gradients' device")
+        wsb = lib.cfd_grad_norm_workspace_bytes(sizes, n)
+        if wsb < 0:
+            check(-1, "cfd_grad_norm_workspace_bytes")
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+        check(lib.cfd_grad_norm(ptrs, sizes, n, _DT[grads[0].dtype], float(max_norm), _ptr(ws), _ptr(out), _stream()), "cfd_grad_norm")
+    return out
+
+
+ADAMW_BLOCK = 256      # elements that share a scale of an 8-bit state; every tensor's state segment is padded to it
+
+
+def adamw_step(table, desc: AdamwDesc, m, v, m_scale, v_scale, t, lr, grad_scale, ws) -> None:
+    """cfd_adamw_step on a host table of AdamwTensor records; trainer.AdamW builds and checks the operands"""
+    with _on(m.device):
+        check(_lib.load().cfd_adamw_step(table, len(table), C.byref(desc), _ptr(m), _ptr(v), _ptr(m_scale), _ptr(v_scale), _ptr(t),
+                                         _ptr(lr), _ptr(grad_scale), _ptr(ws), _stream()), "cfd_adamw_step")
+
+
+# ----------------------------------------------------------------------------------------
+# 4-bit microscaled matrices and the Dense layer on them
+# ----------------------------------------------------------------------------------------
+class Mxfp4(NamedTuple):
+    """rows x cols matrix in 4 bits, blocked by 32 along its columns (include/cfd_amd.h): codes uint8 (rows, 16 ceil(cols / 32)),
+    scales uint8 (rows, cfd_mxfp4_scale_pitch(cols)); value = E2M1 code * 2^(scale - 127)"""
+    codes: torch.Tensor
+    scales: torch.Tensor
+    cols: int
+
+    @property
+    def shape(self):
+        return (self.codes.shape[0], self.cols)
+
+
+def _mx_empty(rows: int, cols: int, device) -> Mxfp4:
+    pitch = (cols + 511) // 512 * 16
+    return Mxfp4(torch.empty((rows, (cols + 31) // 32 * 16), dtype=torch.uint8, device=device),
+                 torch.empty((rows, pitch), dtype=torch.uint8, device=device), cols)
+
+
+def _mx_check(q: Mxfp4, what: str) -> None:
+    _need(isinstance(q, Mxfp4), f"{what} must be an Mxfp4 matrix")
+    _need(0 < q.cols <= 1 << 22, f"{what}: columns must be in 1 .. 4194304")
+    nb, rows = (q.cols + 31) // 32, q.codes.shape[0]
+    for t, width, name in ((q.codes, nb * 16, "codes"), (q.scales, (nb + 15) // 16 * 16, "scales")):
+        _dev(t)
+        _need(t.dtype == torch.uint8 and tuple(t.shape) == (rows, width) and t.is_contiguous(),
+              f"{what} {name} must be dense uint8 {(rows, width)}, is {t.dtype} {tuple(t.shape)}")
+    _need(q.codes.device == q.scales.device, f"{what}: codes and scales on one device")
+
+
+def _mx_input(x: torch.Tensor, what: str) -> int:
+    """row stride of a 2-D fp32 / bf16 matrix whose rows are dense"""
+    _dev(x)
+    _need(x.dim() == 2 and x.dtype in _DT, f"{what} must be a 2-D fp32 or bf16 matrix, is {x.dtype} {tuple(x.shape)}")
+    rows, cols = x.shape
+    _need(0 < cols <= 1 << 22, f"{what}: columns must be in 1 .. 4194304")
+    _need((cols == 1 or x.stride(1) == 1) and (rows <= 1 or x.stride(0) >= cols),
+          f"{what} must have dense rows that do not overlap, strides {tuple(x.stride())}")
+    return x.stride(0) if rows > 1 else cols
+
+
+def _mx_quantize(x: torch.Tensor, rows: bool, cols: bool):
+    ldx = _mx_input(x, "mxfp4_quantize: x")
+    R, K = x.shape
+    _need(not cols or 0 < R <= 1 << 22, "mxfp4_quantize: a transposed matrix needs 1 .. 4194304 rows")
+    with _on(x.device):
+        q = _mx_empty(R, K, x.device) if rows else None
+        t = _mx_empty(K, R, x.device) if cols else None
+        check(_lib.load().cfd_mxfp4_quantize(_ptr(x), ldx, _DT[x.dtype], R, K, _ptr(q and q.codes), _ptr(q and q.scales),
+                                             _ptr(t and t.codes), _ptr(t and t.scales), _stream()), "cfd_mxfp4_quantize")
+    return q, t
+
+
+def mxfp4_quantize(x: torch.Tensor, transpose: bool = False) -> Mxfp4:
+    """x (rows, cols) fp32 / bf16 -> 4 bits, blocks along the columns; transpose=True: the (cols, rows) matrix, blocks along
+    x's rows (the operand of a product that contracts over them: a data or weight gradient)"""
+    return _mx_quantize(x, not transpose, transpose)[int(transpose)]
+
+
+def mxfp4_quantize_both(x: torch.Tensor) -> Tuple[Mxfp4, Mxfp4]:
+    """(mxfp4_quantize(x), mxfp4_quantize(x, transpose=True)) from one read of x"""
+    return _mx_quantize(x, True, True)
+
+
+def mxfp4_dequantize(q: Mxfp4, dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """the values of a 4-bit matrix (exact in either dtype, scales at the ends of the exponent range aside)"""
+    _mx_check(q, "mxfp4_dequantize: q")
+    rows, cols = q.shape
+    with _on(q.codes.device):
+        if out is None:
+            out = torch.empty((rows, cols), dtype=dtype, device=q.codes.device)
+        ldy = _mx_input(out, "mxfp4_dequantize: out")
+        _need(tuple(out.shape) == (rows, cols) and out.device == q.codes.device, f"mxfp4_dequantize: out must be {(rows, cols)} on q's device")
+        check(_lib.load().cfd_mxfp4_dequantize(_ptr(q.codes), _ptr(q.scales), rows, cols, _ptr(out), ldy, _DT[out.dtype], _stream()),
+              "cfd_mxfp4_dequantize")
+    return out
+
+
+def mxfp4_from_parts(codes: torch.Tensor, scales: torch.Tensor, cols: int) -> Mxfp4:
+    """an Mxfp4 matrix from packed codes uint8 (rows, 16 * blocks) and one scale byte per block, uint8 (rows, blocks): the
+    scales are laid out once as the kernels read them"""
+    nb = (int(cols) + 31) // 32
+    _dev(codes)
+    _need(codes.dim() == 2 and codes.dtype == torch.uint8 and codes.shape[1] == nb * 16, f"mxfp4_from_parts: codes must be uint8 (rows, {nb * 16})")
+    _need(scales.dtype == torch.uint8 and tuple(scales.shape) == (codes.shape[0], nb) and scales.device == codes.device,
+          f"mxfp4_from_parts: scales must be uint8 {(codes.shape[0], nb)} on the codes' device")
+    laid = torch.zeros((codes.shape[0], (nb + 15) // 16 * 16), dtype=torch.uint8, device=codes.device)
+    laid[:, :nb] = scales
+    codes = codes.contiguous()
+    tail = int(cols) % 32
+    if tail:                        # codes past the last column are zero
+        codes = codes.clone()
+        codes[:, (nb - 1) * 16 + (tail + 1) // 2:] = 0
+        if tail % 2:
+            codes[:, (nb - 1) * 16 + tail // 2] &= 15
+    return Mxfp4(codes, laid, int(cols))
+
+
+def mxfp4_dense(x: Union[Mxfp4, torch.Tensor], w: Mxfp4, bias: Optional[torch.Tensor] = None, act: int = ACT_NONE,
+                out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None, slope: float = LEAKY_SLOPE) -> torch.Tensor:
+    """y (m, n) = act(x w^T + bias), fp32 accumulation.  w: (n, k) in 4 bits.  x: (m, k) in 4 bits -- both operands on the
+    4-bit matrix instructions, for training and large batches -- or fp32 / bf16, which keeps the activations' precision and
+    reads the weights once (a few rows).  The gradients of y = x w^T are the same product on transposed operands:
+    dx = mxfp4_dense(quantize(dy), quantize(w, transpose=True)), dw = mxfp4_dense(quantize(dy, transpose=True),
+    quantize(x, transpose=True))."""
+    lib = _lib.load()
+    _mx_check(w, "mxfp4_dense: w")
+    n, k = w.shape
+    dev = w.codes.device
+    four = isinstance(x, Mxfp4)
+    if four:
+        _mx_check(x, "mxfp4_dense: x")
+        xt, ldx, kind = x.codes, 0, _lib.MX_X_MXFP4
+    else:
+        xt, ldx = x, _mx_input(x, "mxfp4_dense: x")
+        kind = _lib.MX_X_F32 if x.dtype == torch.float32 else _lib.MX_X_BF16
+    m = x.shape[0]
+    _need(x.shape[1] == k, f"mxfp4_dense: x has {x.shape[1]} columns, w {k}")
+    _need(xt.device == dev and (bias is None or bias.device == dev), "mxfp4_dense: x, w and bias on one device")
+    _numel(bias, n, "mxfp4_dense bias", torch.float32)
+    odt = out_dtype or (out.dtype if out is not None else torch.float32 if four else x.dtype)
+    with _on(dev):
+        if out is None:
+            out = torch.empty((m, n), dtype=odt, device=dev)
+        _need(tuple(out.shape) == (m, n) and out.dtype == odt and odt in _DT and out.device == dev,
+              f"mxfp4_dense: out must be {odt} {(m, n)} on w's device, is {out.dtype} {tuple(out.shape)}")
+        if m == 0 or n == 0:
+            return out
+        d = Mxfp4DenseDesc(x_kind=kind, out_dtype=_DT[odt], act=act, leaky_slope=slope, m=m, n=n, k=k, ldx=ldx,
+                           ldy=_mx_input(out, "mxfp4_dense: out"))
+        wsb = lib.cfd_mxfp4_dense_workspace_bytes(m, n, k, int(not four))
+        if wsb < 0:
+            check(-1, "cfd_mxfp4_dense_workspace_bytes")
+        ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+        check(lib.cfd_mxfp4_dense(C.byref(d), _ptr(xt), _ptr(x.scales) if four else None, _ptr(w.codes), _ptr(w.scales), _ptr(bias),
+                                  _ptr(out), _ptr(ws), _stream()), "cfd_mxfp4_dense")
+    return out

@@ -61,6 +61,95 @@ class Adam:
             self.apply(a, b, g, alpha, grad_scale)
 
 
+class AdamW:
+    """keras.optimizers.AdamW(learning_rate, weight_decay, beta_1, beta_2, epsilon) over a list of tensors, one launch per
+    64 of them, with the state in fp32 (state_bits=32) or in 8 bits with a power-of-two scale per 256 elements (state_bits=8:
+    16 instead of 28 bytes of traffic per fp32 parameter, 2 instead of 8 bytes of state; cfd_adamw_step has the formulas).
+
+    params: dense fp32 or bf16 tensors of one dtype, updated in place; copies: bf16 tensors of the same lengths that receive
+    fp32 parameters as the matrix kernels read them (None: none); weight_decay: one value or one per tensor (0 for
+    biases and BatchNorm, as Keras' exclude_from_weight_decay).  lr is read at every step; an fp32 device tensor of one
+    element may be given instead, for a schedule inside a captured graph.
+
+    State, flat over all tensors (segment i at offsets[i], padded to 256 with zeros), for checkpoints and inspection:
+    m, v (fp32, or float8_e4m3fn / float8_e5m2 codes with m_scale, v_scale fp32: value = code * scale[element // 256]) and
+    t, the int32 device counter of the steps taken.  step() waits for nothing and allocates nothing: it can be captured."""
+
+    def __init__(self, params, lr=1e-3, beta_1: float = 0.9, beta_2: float = ADAM_BETA_2, epsilon: float = ADAM_EPS,
+                 weight_decay=0.004, state_bits: int = 32, copies=None, seed: int = 0):
+        self.params = [params] if isinstance(params, torch.Tensor) else list(params)
+        self.copies = None if copies is None else [copies] if isinstance(copies, torch.Tensor) else list(copies)
+        n = len(self.params)
+        if n == 0:
+            raise ValueError("AdamW needs at least one parameter")
+        ops._tensor_list(self.params, "AdamW: parameters")
+        p0 = self.params[0]
+        self.device = p0.device
+        self.weight_decay = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else [float(d) for d in weight_decay]
+        if len(self.weight_decay) != n:
+            raise ValueError(f"AdamW: {len(self.weight_decay)} weight decays for {n} parameters")
+        if self.copies is not None:
+            if p0.dtype != torch.float32 or len(self.copies) != n:
+                raise ValueError("AdamW: copies need fp32 parameters, one each")
+            ops._tensor_list(self.copies, "AdamW: copies", torch.bfloat16, self.device)
+            if any(c.numel() != p.numel() for c, p in zip(self.copies, self.params)):
+                raise ValueError("AdamW: a copy must have its parameter's length")
+        if state_bits not in (8, 32):
+            raise ValueError("AdamW: state_bits must be 8 or 32")
+        if not (0.0 <= beta_1 < 1.0 and 0.0 <= beta_2 < 1.0 and epsilon >= 0.0):
+            raise ValueError("AdamW: beta must be in [0, 1) and epsilon >= 0")
+        if isinstance(lr, torch.Tensor) and not (lr.device == self.device and lr.dtype == torch.float32 and lr.numel() == 1):
+            raise ValueError("AdamW: a learning-rate tensor must be one fp32 element on the parameters' device")
+        spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in self.params + (self.copies or []) if t.numel())
+        if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+            raise ValueError("AdamW: parameters (and copies) must not overlap")
+        self.lr, self.b1, self.b2, self.eps, self.state_bits, self.seed = lr, beta_1, beta_2, epsilon, state_bits, int(seed)
+        self.offsets, off = [], 0
+        for p in self.params:
+            self.offsets.append(off)
+            off += -(-p.numel() // ops.ADAMW_BLOCK) * ops.ADAMW_BLOCK
+        z = lambda size, dt: torch.zeros(size, dtype=dt, device=self.device)  # noqa: E731
+        dm, dv = (torch.float32, torch.float32) if state_bits == 32 else (torch.float8_e4m3fn, torch.float8_e5m2)
+        self.m, self.v = z(max(off, 16), torch.uint8 if state_bits == 8 else dm), z(max(off, 16), torch.uint8 if state_bits == 8 else dv)
+        self.m, self.v = self.m.view(dm)[:off], self.v.view(dv)[:off]
+        self.m_scale = z(off // ops.ADAMW_BLOCK, torch.float32) if state_bits == 8 else None
+        self.v_scale = z(off // ops.ADAMW_BLOCK, torch.float32) if state_bits == 8 else None
+        self.t = z(1, torch.int32)
+        self._ws = z(32, torch.uint8)
+        self._table = (ops.AdamwTensor * n)()
+        self._desc = ops.AdamwDesc(p_dtype=ops._DT[p0.dtype], state_bits=state_bits, seed=self.seed & 0xffffffff, eps=epsilon,
+                                   beta1=beta_1, beta2=beta_2)
+        self._sizes = [p.numel() for p in self.params]
+        for k, p in enumerate(self.params):
+            e = self._table[k]
+            e.p, e.n, e.state_offset, e.weight_decay = p.data_ptr(), p.numel(), self.offsets[k], self.weight_decay[k]
+            e.copy = self.copies[k].data_ptr() if self.copies is not None else None
+        self._ptrs = self._addresses()
+
+    def _addresses(self):
+        return [t.data_ptr() for t in self.params + (self.copies or [])]
+
+    def step(self, grads, grad_scale=None) -> None:
+        """One update from `grads` (one dense fp32 or bf16 tensor per parameter, one dtype).  grad_scale: None, or an fp32
+        device tensor of one element that multiplies every gradient (ops.grad_norm(...)[1:]); where it is not finite the
+        whole step is skipped, t included."""
+        grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+        if [g.numel() for g in grads] != self._sizes:
+            raise ValueError("AdamW.step: one gradient per parameter, of its length")
+        ops._tensor_list(grads, "AdamW.step: gradients", None, self.device)
+        if self._addresses() != self._ptrs:
+            raise RuntimeError("AdamW: a parameter's storage was replaced after the optimizer was built")
+        if grad_scale is not None and not (grad_scale.device == self.device and grad_scale.dtype == torch.float32 and grad_scale.numel() == 1):
+            raise ValueError("AdamW.step: grad_scale must be one fp32 element on the parameters' device")
+        for e, g in zip(self._table, grads):
+            e.g = g.data_ptr()
+        self._desc.g_dtype = ops._DT[grads[0].dtype]
+        on_device = isinstance(self.lr, torch.Tensor)
+        self._desc.lr = 0.0 if on_device else float(self.lr)
+        ops.adamw_step(self._table, self._desc, self.m, self.v, self.m_scale, self.v_scale, self.t, self.lr if on_device else None,
+                       grad_scale, self._ws)
+
+
 def _cast(src: torch.Tensor, dst: torch.Tensor) -> None:
     """dst <- src across dtypes (bf16 gradient exchange): the library's cast kernel on the GPU, torch on CPU tensors
     (the gloo tests)"""

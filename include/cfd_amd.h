@@ -315,6 +315,73 @@ int cfd_field_loss(const float *y, const float *target, int64_t n, int kind, flo
  * w_compute (may be NULL): the bf16 shadow copy of w, refreshed in the same pass. */
 int cfd_adam_step(float *w, const float *g, float *m, float *v, void *w_compute, int compute_dtype, int64_t n,
                   float alpha, float beta1, float beta2, float eps, float grad_scale, void *stream);
+/* ---- optimizer over a list of tensors (no counterpart in the reference, which uses Adam; same Keras form as
+ * cfd_adam_step).  Arrays of pointers, lengths and tensor records are HOST arrays; what they point to is device memory.
+ *
+ * Global L2 norm of `count` gradients g[i] of n[i] elements (n[i] may be 0; one dtype for all, any alignment) and the factor
+ * that clips it: out[0] = norm, out[1] = min(1, max_norm / norm), or NaN where the norm is not finite.  Squares and
+ * sums in fp64, in a fixed order.  ws: cfd_grad_norm_workspace_bytes(n, count) bytes, 8-byte aligned. */
+int64_t cfd_grad_norm_workspace_bytes(const int64_t *n, int count);
+int cfd_grad_norm(const void *const *g, const int64_t *n, int count, int dtype, float max_norm, void *ws, float *out,
+                  void *stream);
+
+/* One AdamW step over `count` tensors in one launch per 64 of them:
+ *   t = ++*step;  alpha = lr sqrt(1-b2^t)/(1-b1^t);  g' = g*gs;  m += (g'-m)(1-b1);  v += (g'^2-v)(1-b2);
+ *   p -= p*lr*weight_decay;  p -= alpha*m/(sqrt(v)+eps);  copy (bf16, may be NULL) = p
+ * gs = *grad_scale (device, e.g. out + 1 of cfd_grad_norm; NULL = 1).  A gs that is not finite skips the whole step, *step
+ * included.  lr_device (may be NULL): the learning rate is read from the device instead of from the descriptor.
+ * step, lr_device and grad_scale live on the device, so a captured graph advances on every replay.  ws: 32 bytes.
+ *   state_bits 32: m, v fp32 [state elements]; m_scale, v_scale unused.
+ *   state_bits  8: m e4m3 codes, v e5m2 codes [state elements], m_scale, v_scale fp32 [state elements / 256]: the value
+ *     is code * scale[element / 256].  Stored by stochastic rounding from a hash of (seed, t, position): the expected
+ *     state is the 32-bit recursion's; v > 0 never rounds to 0.  A block of 256 with an infinity or NaN gets a NaN scale.
+ * Tensor i's state starts at state_offset (a multiple of 256; its segment is padded to one with zeros).  Tensors and
+ * their state segments must not overlap. */
+typedef struct {
+  void *p;             /* p_dtype [n] */
+  const void *g;       /* g_dtype [n] */
+  void *copy;          /* bf16 [n] or NULL (needs fp32 p) */
+  int64_t n;           /* may be 0 */
+  int64_t state_offset;
+  float weight_decay;
+} cfd_adamw_tensor;
+typedef struct {
+  int p_dtype, g_dtype; /* cfd_dtype */
+  int state_bits;       /* 32 or 8 */
+  unsigned seed;        /* of the 8-bit state's rounding */
+  float lr, eps;
+  double beta1, beta2;
+} cfd_adamw_desc;
+int cfd_adamw_step(const cfd_adamw_tensor *tensors, int count, const cfd_adamw_desc *desc, void *m, void *v, float *m_scale,
+                   float *v_scale, int *step, const float *lr_device, const float *grad_scale, void *ws, void *stream);
+
+/* ---- 4-bit microscaled matrices (OCP MX: E2M1 codes, an E8M0 power of two per 32) and the Dense layer on them (no
+ * counterpart in the reference; the Dense layers are DeltaP/models/generator.py:40-46).  A matrix of `rows` x `cols` blocked along its columns is
+ *   codes  uint8 [rows][16 * ceil(cols / 32)], low nibble = lower column, zero past cols;
+ *   scales uint8 [rows][cfd_mxfp4_scale_pitch(cols)], value 2^(byte - 127), 255 = NaN, zero past the last block.
+ * Both arrays start 16-byte aligned.  1 <= cols <= 4194304; rows may be 0.
+ *
+ * cfd_mxfp4_quantize: x [rows][ldx >= cols] fp32 / bf16 -> codes, scales (blocks along the columns) and / or codes_t, scales_t
+ * (blocks along the rows: the transposed matrix, cols rows of `rows` columns); a pair may be NULL.  Scale: floor(log2 max) - 2,
+ * one more where max > 7 * 2^that; codes round to nearest even; a block with an infinity or NaN becomes NaN. */
+int64_t cfd_mxfp4_scale_pitch(int64_t cols);
+int cfd_mxfp4_quantize(const void *x, int64_t ldx, int dtype, int64_t rows, int64_t cols, uint8_t *codes, uint8_t *scales,
+                       uint8_t *codes_t, uint8_t *scales_t, void *stream);
+int cfd_mxfp4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t cols, void *y, int64_t ldy, int dtype,
+                         void *stream);
+/* y [m][ldy >= n] = act(x w^T + bias), fp32 accumulation.  w: n x k in 4 bits; x: m x k in 4 bits (codes in `x`, x_scales) or
+ * float (x [m][ldx >= k], x_scales NULL): then the weights are read once and the activations keep their precision --
+ * the form for a few rows.  bias fp32 [n] or NULL.  ws: cfd_mxfp4_dense_workspace_bytes bytes (may be 0). */
+typedef enum { CFD_MX_X_F32 = 0, CFD_MX_X_BF16 = 1, CFD_MX_X_MXFP4 = 2 } cfd_mxfp4_x_kind;
+typedef struct {
+  int x_kind, out_dtype, act;
+  float leaky_slope;
+  int64_t m, n, k, ldx, ldy;
+} cfd_mxfp4_dense_desc;
+int64_t cfd_mxfp4_dense_workspace_bytes(int64_t m, int64_t n, int64_t k, int x_float);
+int cfd_mxfp4_dense(const cfd_mxfp4_dense_desc *desc, const void *x, const uint8_t *x_scales, const uint8_t *w_codes,
+                    const uint8_t *w_scales, const float *bias, void *y, void *ws, void *stream);
+
 /* moving = moving*momentum + batch*(1-momentum), once per sample in order (BatchNormalization momentum 0.99) */
 int cfd_bn_update_moving(float *moving_mean, float *moving_var, const float *mean, const float *var, int B, int C,
                          float momentum, void *stream);
