@@ -197,6 +197,7 @@ struct MxDense {
   int mt, nt;
   int out_bf16, act;
   float slope;
+  bool big;                           // 256 x 256 tiles
 };
 
 __device__ __forceinline__ void mx_store(const MxDense &p, int64_t m, int n, float v) {   // one element of the output
@@ -284,6 +285,222 @@ __global__ __launch_bounds__(256) void mx_dense_kernel(MxDense p) {
   for (int j = 0; j < 2; ++j)
 #pragma unroll
     for (int i = 0; i < 2; ++i) mx_emit(p, sk, m0 + wm + j * 16 + fr, n0 + wn + i * 16 + fq * 4, acc[i][j]);
+}
+
+// Large products: 256 (n) x 256 (m) tile, eight waves in two groups that run one barrier apart, so that on every SIMD one
+// wave feeds the matrix cores while the other reads fragments and issues loads.
+//   * a K tile is 256 columns = 128 bytes a row; it is staged as four half tiles of 128 rows (A0, B0, B1, A1; 16 KiB each), two
+//     stages, by LDS-DMA that stays in flight across barriers; 16-byte chunks are XOR-ed with the row's low three bits;
+//   * wave (wr, wc) owns n rows wr*64 + [0, 64) of both A halves and m rows wc*32 + [0, 32) of both B halves: 4 x 2 fragments of
+//     32 x 32, 128 accumulator registers; 32x32x64 scaled MFMA, lane = row l & 31, k half l >> 5; step s of a K tile takes
+//     block 4 (l >> 5) + s, so one 32-bit word holds a lane's four scales of the K tile and the step picks the byte;
+//   * scales: 16 bytes a row cover two K tiles; one LDS-DMA load per wave every second K tile (8 KiB, two stages);
+//   * two phases a K tile: read A0, B0, B1, issue B1', A1', 16 MFMAs; read A1, issue A0'', B0'', 16 MFMAs.
+// Codes behind the last column need no mask: their scale bytes are zero on both operands and 2^-254 is zero in fp32.
+constexpr int MXT_HALF = 128 * 128, MXT_STAGE = 4 * MXT_HALF, MXT_SCALE = 2 * MXT_STAGE, MXT_SCALE_STAGE = 512 * 16;
+constexpr int MXT_LDS = MXT_SCALE + 2 * MXT_SCALE_STAGE;   // 144 KiB
+constexpr int MXT_ROW = 528;                               // staged output: 512 bytes a row and a pad that spreads the banks
+static_assert(256 * MXT_ROW <= MXT_LDS, "the staged output reuses the stages");
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x4a2 __attribute__((ext_vector_type(4), aligned(2)));
+
+__device__ __forceinline__ void mx_dma16(__amdgpu_buffer_rsrc_t r, unsigned voff, unsigned soff, char *dst) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)dst, 16, (int)voff, (int)soff, 0, 0);
+}
+template <int N> __device__ __forceinline__ void mx_wait() {
+  static_assert(N == 0 || N == 6 || N == 8 || N == 9, "counts that the schedule uses");
+  if constexpr (N == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  else if constexpr (N == 6) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
+  else if constexpr (N == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
+}
+
+// tile of a workgroup: each XCD gets a contiguous run of tiles (it has its own L2), and runs walk 8 m tiles before the next
+// n tile, so the ~32 tiles an XCD works on at once span 8 x 4 operand panels instead of 2 x 16
+__device__ __forceinline__ void mx_tile_of(const MxDense &p, int &mt, int &nt, int &sk) {
+  const int nwg = p.mt * p.nt * p.split, q = nwg >> 3, r = nwg & 7, xcd = blockIdx.x & 7;
+  int t = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + ((int)blockIdx.x >> 3);
+  sk = t / (p.mt * p.nt);
+  t -= sk * p.mt * p.nt;
+  const int g = t / (8 * p.nt), h = min(8, p.mt - g * 8), u = t - g * 8 * p.nt;
+  nt = u / h;
+  mt = g * 8 + u - nt * h;
+}
+
+template <typename TO> __global__ __launch_bounds__(512, 2) void mx_dense256_kernel(MxDense p) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave >> 2, wc = wave & 3;
+  int mt, nt, sk;
+  mx_tile_of(p, mt, nt, sk);
+  const int m0 = mt * 256, n0 = nt * 256, cp = p.nb * 16;
+  const int mr = min(256, p.M - m0), nr = min(256, p.N - n0);
+  // K in pairs of tiles; a pair may end behind the last block (its scales are zero there)
+  const int kbeg = sk * p.kt_per, pairs = (min(kbeg + p.kt_per, (p.nb + 7) / 8) - kbeg + 1) / 2;   // kt_per is even
+  const __amdgpu_buffer_rsrc_t xr = mx_rsrc(p.xc, m0, mr, cp), wres = mx_rsrc(p.wc, n0, nr, cp);
+  // waves 0..3 stage the scales of the 256 weight rows, 4..7 those of the activations
+  const __amdgpu_buffer_rsrc_t sres = wr ? mx_rsrc(p.xs, m0, mr, p.pitch) : mx_rsrc(p.ws, n0, nr, p.pitch);
+  const unsigned soff = (unsigned)((wc * 64 + lane) * p.pitch);
+
+  // half tile = 16 wave loads of 8 rows; wave w issues pieces w and 8 + w; lane -> row lane / 8, source chunk swizzled
+  const int lrow = lane >> 3, chunk = (lane & 7) ^ lrow;
+  unsigned voff[4];   // half * 2 + piece
+#pragma unroll
+  for (int r = 0; r < 4; ++r) voff[r] = (unsigned)(((r >> 1) * 128 + (r & 1) * 64 + wave * 8 + lrow) * cp + chunk * 16);
+  int left = pairs * 2, spairs = pairs;
+  unsigned koff = (unsigned)kbeg * 128, spair = (unsigned)kbeg * 8;
+  char *const dmaw = lds + wave * 1024;
+  auto issue = [&](int slot, int stage) {
+    char *dst = dmaw + stage * MXT_STAGE + slot * MXT_HALF;
+    const __amdgpu_buffer_rsrc_t rs = (slot == 0 || slot == 3) ? wres : xr;
+    const int h = slot >> 1;   // A0, B0 | B1, A1
+    mx_dma16(rs, voff[h * 2], koff, dst);
+    mx_dma16(rs, voff[h * 2 + 1], koff, dst + 8192);
+  };
+  auto advance = [&]() { if (left > 1) { --left; koff += 128; } };   // past the end the last K tile is issued again
+  auto issue_scales = [&](int stage) { mx_dma16(sres, soff, spair, lds + MXT_SCALE + stage + wave * 1024); };
+  int sst = 0;   // scale stage of the current pair (byte offset)
+  auto advance_scales = [&]() { if (spairs > 1) { --spairs; spair += 16; } };
+
+  const int fr = lane & 31, fh = lane >> 5;
+  const int laneoff = fr * 128 + (((fh * 4) ^ (fr & 7)) << 4);
+  const char *ard[4], *brd[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+    ard[s] = lds + ((wr * 64 * 128 + laneoff) ^ (s << 4));
+    brd[s] = lds + ((wc * 32 * 128 + laneoff) ^ (s << 4));
+  }
+  const char *asc = lds + MXT_SCALE + (wr * 64 + fr) * 16 + fh * 4, *bsc = lds + MXT_SCALE + (256 + wc * 32 + fr) * 16 + fh * 4;
+
+  f32x16 acc[4][2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+
+  issue_scales(0); advance_scales();
+#pragma unroll
+  for (int h = 0; h < 6; ++h) {
+    issue(h & 3, (h >> 2) & 1);
+    if ((h & 3) == 3) advance();
+  }
+  mx_wait<6>();
+  __builtin_amdgcn_s_barrier();
+  if (wr == 1) __builtin_amdgcn_s_barrier();   // the second group runs one barrier behind
+
+  i32x4 a[2][4], b[2][4];
+  int as[2], bs[2];
+#define MX_READ_A(ST, SLOT, HALF)                                                                       \
+  _Pragma("unroll") for (int s = 0; s < 4; ++s)                                                         \
+    _Pragma("unroll") for (int i = 0; i < 2; ++i)                                                       \
+      a[i][s] = *(const i32x4 *)(ard[s] + ST * MXT_STAGE + SLOT * MXT_HALF + i * 32 * 128);       \
+  _Pragma("unroll") for (int i = 0; i < 2; ++i)                                                         \
+    as[i] = *(const int *)(asc + (HALF * 128 + i * 32) * 16 + ST * 8);
+#define MX_READ_B(ST)                                                                                   \
+  _Pragma("unroll") for (int s = 0; s < 4; ++s)                                                         \
+    _Pragma("unroll") for (int j = 0; j < 2; ++j)                                                       \
+      b[j][s] = *(const i32x4 *)(brd[s] + ST * MXT_STAGE + (1 + j) * MXT_HALF);                   \
+  _Pragma("unroll") for (int j = 0; j < 2; ++j)                                                         \
+    bs[j] = *(const int *)(bsc + j * 128 * 16 + ST * 8);
+#define MX_STEP(AI, S)                                                                                  \
+  _Pragma("unroll") for (int i = 0; i < 2; ++i)                                                         \
+    _Pragma("unroll") for (int j = 0; j < 2; ++j)                                                       \
+      acc[AI + i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a[i][S]), wide(b[j][S]), acc[AI + i][j], 4, 4, S, as[i], S, bs[j]);
+#define MX_MFMAS(AI) MX_STEP(AI, 0) MX_STEP(AI, 1) MX_STEP(AI, 2) MX_STEP(AI, 3)
+#define MX_SYNC(N)                                                                                      \
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                                                    \
+  mx_wait<N>();                                                                                         \
+  __builtin_amdgcn_s_barrier();                                                                         \
+  __builtin_amdgcn_sched_barrier(0);                                                                    \
+  __builtin_amdgcn_s_setprio(1);
+#define MX_END                                                                                          \
+  __builtin_amdgcn_s_setprio(0);                                                                        \
+  __builtin_amdgcn_sched_barrier(0);                                                                    \
+  __builtin_amdgcn_s_barrier();
+// ST: K tile of the pair = code stage and half of the scale row; the first also issues the next pair's scales
+#define MX_KTILE(ST)                                                                                    \
+  {                                                                                                     \
+    MX_READ_A(ST, 0, 0) MX_READ_B(ST)                                                                   \
+    if constexpr (ST == 0) { issue_scales(sst ^ MXT_SCALE_STAGE); advance_scales(); }                   \
+    issue(2, 1 - ST); issue(3, 1 - ST); advance();                                                      \
+    MX_SYNC((ST ? 8 : 9))                                                                         \
+    MX_MFMAS(0)                                                                                         \
+    MX_END                                                                                              \
+    MX_READ_A(ST, 3, 1)                                                                                 \
+    issue(0, ST); issue(1, ST);                                                                 \
+    MX_SYNC(6)                                                                                          \
+    MX_MFMAS(2)                                                                                         \
+    MX_END                                                                                              \
+  }
+  for (int k = 0; k < pairs; ++k) {
+    MX_KTILE(0)
+    MX_KTILE(1)
+    sst ^= MXT_SCALE_STAGE;
+    asc = lds + ((unsigned)(asc - lds) ^ MXT_SCALE_STAGE);
+    bsc = lds + ((unsigned)(bsc - lds) ^ MXT_SCALE_STAGE);
+  }
+#undef MX_KTILE
+#undef MX_END
+#undef MX_SYNC
+#undef MX_MFMAS
+#undef MX_STEP
+#undef MX_READ_B
+#undef MX_READ_A
+  if (wr == 0) __builtin_amdgcn_s_barrier();
+  mx_wait<0>();        // the tail loads must have landed before the stages are reused
+  __syncthreads();
+
+  // epilogue: lane holds n = 8q + 4 fh + r (q, r < 4) of fragment row i, pixel row m = fr of fragment j; through LDS, so
+  // that whole 512-byte runs of an output row leave together (fp32: two passes of 128 columns)
+  constexpr int ES = sizeof(TO), NPASS = ES / 2, COLS = 256 / NPASS, EPC = 16 / ES;
+  const bool raw = p.split > 1;
+  TO *const y = raw ? (TO *)p.slab + (int64_t)sk * p.M * p.N : (TO *)p.y;
+  const int64_t ldy = raw ? p.N : p.ldy;
+#pragma unroll
+  for (int h = 0; h < NPASS; ++h) {
+    if (h) __syncthreads();
+#pragma unroll
+    for (int ii = 0; ii < 4 / NPASS; ++ii) {
+      const int i = h * 2 + ii;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int nl = (i >> 1) * 128 + wr * 64 + (i & 1) * 32 + q * 8 + fh * 4;
+        f32x4 bv = {0.f, 0.f, 0.f, 0.f};
+        if (p.bias && !raw) {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (n0 + nl + r < p.N) bv[r] = p.bias[n0 + nl + r];
+        }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          TO o[4];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            const float v = acc[i][j][q * 4 + r] + bv[r];
+            o[r] = (TO)(raw ? v : apply_act(v, p.act, p.slope));
+          }
+          char *d = lds + (j * 128 + wc * 32 + fr) * MXT_ROW + (nl - h * COLS) * ES;
+          if constexpr (ES == 2) *(bf16x4 *)d = (bf16x4){o[0], o[1], o[2], o[3]};
+          else *(f32x4 *)d = (f32x4){o[0], o[1], o[2], o[3]};
+        }
+      }
+    }
+    __syncthreads();
+    const int c = (lane & 31) * EPC, n = n0 + h * COLS + c;
+#pragma unroll 4
+    for (int it = 0; it < 16; ++it) {
+      const int ml = wave * 32 + it * 2 + (lane >> 5);
+      if (ml >= mr || n >= p.N) continue;
+      const char *src = lds + ml * MXT_ROW + c * ES;
+      TO *dst = y + (int64_t)(m0 + ml) * ldy + n;
+      if (n + EPC <= p.N) *(u32x4a2 *)dst = *(const u32x4a2 *)src;
+      else
+        for (int e = 0; e < p.N - n; ++e) dst[e] = ((const TO *)src)[e];
+    }
+  }
 }
 
 // Float activations against 4-bit weights (serving: the weights are what is read).  A wave owns 64 weight rows x 16
@@ -398,6 +615,18 @@ static void mx_split(MxDense &p, int groups, int64_t tiles, int least) {
 static void mx_plan(MxDense &p, bool serve) {
   p.nb = (int)mx_blocks(p.K);
   p.pitch = (int)mx_scale_pitch(p.K);
+  p.big = !serve && p.M > 128 && p.N > 128;
+  if (p.big) {
+    p.nt = (p.N + 255) / 256;
+    p.mt = (p.M + 255) / 256;
+    const int groups = (p.nb + 7) / 8;
+    int64_t want = 256 / ((int64_t)p.nt * p.mt);
+    if (want > groups / 8) want = groups / 8;
+    if (want < 1) want = 1;
+    p.kt_per = (int)(((groups + want - 1) / want + 1) / 2 * 2);   // whole pairs of K tiles
+    p.split = (groups + p.kt_per - 1) / p.kt_per;
+    return;
+  }
   p.nt = (p.N + 63) / 64;
   p.mt = serve ? (p.M + 15) / 16 : (p.M + 63) / 64;
   mx_split(p, serve ? (p.nb + 15) / 16 : (p.nb + 7) / 8, (int64_t)p.nt * p.mt, 4);
@@ -495,7 +724,13 @@ extern "C" int cfd_mxfp4_dense(const cfd_mxfp4_dense_desc *d, const void *x, con
   const int64_t blocks = (int64_t)p.mt * p.nt * p.split;
   CFD_REQUIRE(blocks <= 0x7fffffff, "too many tiles");
   hipStream_t st = (hipStream_t)stream;
-  if (d->x_kind == CFD_MX_X_MXFP4) hipLaunchKernelGGL(mx_dense_kernel, dim3((unsigned)blocks), dim3(256), 0, st, p);
+  if (p.big) {
+    const bool b16 = p.out_bf16 && p.split == 1;
+    const void *fn = b16 ? (const void *)mx_dense256_kernel<bf16> : (const void *)mx_dense256_kernel<float>;
+    if (int rc = set_max_lds(fn, MXT_LDS)) return rc;
+    if (b16) hipLaunchKernelGGL(mx_dense256_kernel<bf16>, dim3((unsigned)blocks), dim3(512), MXT_LDS, st, p);
+    else hipLaunchKernelGGL(mx_dense256_kernel<float>, dim3((unsigned)blocks), dim3(512), MXT_LDS, st, p);
+  } else if (d->x_kind == CFD_MX_X_MXFP4) hipLaunchKernelGGL(mx_dense_kernel, dim3((unsigned)blocks), dim3(256), 0, st, p);
   else if (d->x_kind == CFD_MX_X_BF16) hipLaunchKernelGGL(mx_serve_kernel<bf16>, dim3((unsigned)blocks), dim3(256), 0, st, p);
   else hipLaunchKernelGGL(mx_serve_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, st, p);
   CFD_LAUNCH_CHECK();
