@@ -8,6 +8,7 @@
 // a spacing at its block's top (the plain floor would clip a block's largest values by up to a quarter); codes round to
 // nearest even.  A block with an infinity or NaN gets the scale 0xFF: the whole block reads as NaN.
 #include "common.h"
+#include <type_traits>
 
 namespace cfd {
 
@@ -287,20 +288,23 @@ __global__ __launch_bounds__(256) void mx_dense_kernel(MxDense p) {
     for (int i = 0; i < 2; ++i) mx_emit(p, sk, m0 + wm + j * 16 + fr, n0 + wn + i * 16 + fq * 4, acc[i][j]);
 }
 
-// Large products: 256 (n) x 256 (m) tile, eight waves in two groups that run one barrier apart, so that on every SIMD one
-// wave feeds the matrix cores while the other reads fragments and issues loads.
-//   * a K tile is 256 columns = 128 bytes a row; it is staged as four half tiles of 128 rows (A0, B0, B1, A1; 16 KiB each), two
-//     stages, by LDS-DMA that stays in flight across barriers; 16-byte chunks are XOR-ed with the row's low three bits;
-//   * wave (wr, wc) owns n rows wr*64 + [0, 64) of both A halves and m rows wc*32 + [0, 32) of both B halves: 4 x 2 fragments of
-//     32 x 32, 128 accumulator registers; 32x32x64 scaled MFMA, lane = row l & 31, k half l >> 5; step s of a K tile takes
-//     block 4 (l >> 5) + s, so one 32-bit word holds a lane's four scales of the K tile and the step picks the byte;
-//   * scales: 16 bytes a row cover two K tiles; one LDS-DMA load per wave every second K tile (8 KiB, two stages);
-//   * two phases a K tile: read A0, B0, B1, issue B1', A1', 16 MFMAs; read A1, issue A0'', B0'', 16 MFMAs.
-// Codes behind the last column need no mask: their scale bytes are zero on both operands and 2^-254 is zero in fp32.
-constexpr int MXT_HALF = 128 * 128, MXT_STAGE = 4 * MXT_HALF, MXT_SCALE = 2 * MXT_STAGE, MXT_SCALE_STAGE = 512 * 16;
+// Large products: 256 (n) x 256 (m) tile, four waves of 128 x 128 (one per SIMD, 256 accumulators in the accumulation
+// registers).  LDS bandwidth decides the wave tile: a 256-column step of eight 128 x 64 waves reads 192 KiB and stages 64 KiB, as
+// long as its MFMAs take at 128 B/clk; four 128 x 128 waves read 128 KiB.
+//   * a K tile is 256 columns = 128 bytes a row (whole cache lines: 64-byte rows filled LDS a quarter slower), two stages for each
+//     operand, filled by LDS-DMA that stays in flight across barriers; 16-byte chunks are XOR-ed with the row's low three bits;
+//   * 32x32x64 scaled MFMA, lane = row l & 31, K half h = l >> 5; step s of a K tile takes block 4h + s, so one 32-bit word holds a
+//     lane's four scales of the K tile and the step picks the byte;
+//   * scales: 16 bytes a row cover two K tiles (8 KiB, two stages, two LDS-DMA loads per wave every second K tile);
+//   * a wave holds its 128 activation rows of the K tile in registers and walks its weight rows 32 at a time: 16 MFMAs, between which
+//     it reads the next 32 weight rows and a part of the next K tile's activations.  Two barriers per K tile: behind the first
+//     the activations' other stage is free, behind the second the weights', and each is refilled a whole K tile ahead of its use.
+// The K range goes in groups of two K tiles; codes behind the last column need no mask: their scale bytes are zero on both
+// operands, and 2^-254 is zero in fp32.  Reads past the operand are cut off by the buffer's size, which shrinks as its base advances.
+constexpr int MXT_OPER = 256 * 128, MXT_SCALE = 4 * MXT_OPER, MXT_SCALE_STAGE = 512 * 16;   // W0, W1, X0, X1, scales
 constexpr int MXT_LDS = MXT_SCALE + 2 * MXT_SCALE_STAGE;   // 144 KiB
 constexpr int MXT_ROW = 528;                               // staged output: 512 bytes a row and a pad that spreads the banks
-static_assert(256 * MXT_ROW <= MXT_LDS, "the staged output reuses the stages");
+static_assert(256 * MXT_ROW + 1024 <= MXT_LDS, "the staged output and the bias reuse the stages");
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef unsigned u32x4a2 __attribute__((ext_vector_type(4), aligned(2)));
@@ -308,12 +312,21 @@ typedef unsigned u32x4a2 __attribute__((ext_vector_type(4), aligned(2)));
 __device__ __forceinline__ void mx_dma16(__amdgpu_buffer_rsrc_t r, unsigned voff, unsigned soff, char *dst) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)dst, 16, (int)voff, (int)soff, 0, 0);
 }
+// one 32x32x64 step; the scale byte is an immediate of the instruction (s is a constant after unrolling)
+__device__ __forceinline__ f32x16 mx_mma(int s, i32x4 a, i32x4 b, f32x16 c, int as, int bs) {
+  switch (s) {
+    case 0: return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a), wide(b), c, 4, 4, 0, as, 0, bs);
+    case 1: return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a), wide(b), c, 4, 4, 1, as, 1, bs);
+    case 2: return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a), wide(b), c, 4, 4, 2, as, 2, bs);
+    default: return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a), wide(b), c, 4, 4, 3, as, 3, bs);
+  }
+}
 template <int N> __device__ __forceinline__ void mx_wait() {
-  static_assert(N == 0 || N == 6 || N == 8 || N == 9, "counts that the schedule uses");
+  static_assert(N == 0 || N == 8 || N == 10 || N == 18, "counts that the schedule uses");
   if constexpr (N == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  else if constexpr (N == 6) asm volatile("s_waitcnt vmcnt(6)" ::: "memory");
   else if constexpr (N == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-  else asm volatile("s_waitcnt vmcnt(9)" ::: "memory");
+  else if constexpr (N == 10) asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(18)" ::: "memory");
 }
 
 // tile of a workgroup: each XCD gets a contiguous run of tiles (it has its own L2), and runs walk 8 m tiles before the next
@@ -325,131 +338,149 @@ __device__ __forceinline__ void mx_tile_of(const MxDense &p, int &mt, int &nt, i
   t -= sk * p.mt * p.nt;
   const int g = t / (8 * p.nt), h = min(8, p.mt - g * 8), u = t - g * 8 * p.nt;
   nt = u / h;
-  mt = g * 8 + u - nt * h;
+  mt = __builtin_amdgcn_readfirstlane(g * 8 + u - nt * h);   // (uniform: said so, or buffer descriptors go through loops)
+  nt = __builtin_amdgcn_readfirstlane(nt);
+  sk = __builtin_amdgcn_readfirstlane(sk);
 }
 
-template <typename TO> __global__ __launch_bounds__(512, 2) void mx_dense256_kernel(MxDense p) {
+template <typename TO> __global__ __launch_bounds__(256, 1) void mx_dense256_kernel(MxDense p) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave >> 2, wc = wave & 3;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave >> 1, wc = wave & 1;
   int mt, nt, sk;
   mx_tile_of(p, mt, nt, sk);
   const int m0 = mt * 256, n0 = nt * 256, cp = p.nb * 16;
   const int mr = min(256, p.M - m0), nr = min(256, p.N - n0);
-  // K in pairs of tiles; a pair may end behind the last block (its scales are zero there)
-  const int kbeg = sk * p.kt_per, pairs = (min(kbeg + p.kt_per, (p.nb + 7) / 8) - kbeg + 1) / 2;   // kt_per is even
-  const __amdgpu_buffer_rsrc_t xr = mx_rsrc(p.xc, m0, mr, cp), wres = mx_rsrc(p.wc, n0, nr, cp);
-  // waves 0..3 stage the scales of the 256 weight rows, 4..7 those of the activations
-  const __amdgpu_buffer_rsrc_t sres = wr ? mx_rsrc(p.xs, m0, mr, p.pitch) : mx_rsrc(p.ws, n0, nr, p.pitch);
-  const unsigned soff = (unsigned)((wc * 64 + lane) * p.pitch);
+  const int gbeg = sk * p.kt_per, groups = min(gbeg + p.kt_per, p.pitch / 16) - gbeg;   // of two K tiles = 512 columns
 
-  // half tile = 16 wave loads of 8 rows; wave w issues pieces w and 8 + w; lane -> row lane / 8, source chunk swizzled
-  const int lrow = lane >> 3, chunk = (lane & 7) ^ lrow;
-  unsigned voff[4];   // half * 2 + piece
+  // ---- staging: a wave fills 64 rows of each operand, eight loads of 8 rows; lane -> row lane / 8, source chunk swizzled
+  unsigned voff[8];
 #pragma unroll
-  for (int r = 0; r < 4; ++r) voff[r] = (unsigned)(((r >> 1) * 128 + (r & 1) * 64 + wave * 8 + lrow) * cp + chunk * 16);
-  int left = pairs * 2, spairs = pairs;
-  unsigned koff = (unsigned)kbeg * 128, spair = (unsigned)kbeg * 8;
-  char *const dmaw = lds + wave * 1024;
-  auto issue = [&](int slot, int stage) {
-    char *dst = dmaw + stage * MXT_STAGE + slot * MXT_HALF;
-    const __amdgpu_buffer_rsrc_t rs = (slot == 0 || slot == 3) ? wres : xr;
-    const int h = slot >> 1;   // A0, B0 | B1, A1
-    mx_dma16(rs, voff[h * 2], koff, dst);
-    mx_dma16(rs, voff[h * 2 + 1], koff, dst + 8192);
+  for (int q = 0; q < 8; ++q) voff[q] = (unsigned)((wave * 64 + q * 8 + (lane >> 3)) * cp + (((lane & 7) ^ (lane >> 3)) << 4));
+  struct Stream {      // one operand: base of the next K tile, bytes from there to the operand's end, K tiles not issued yet
+    const uint8_t *at;
+    int left, todo;
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t rsrc() const {
+      return __builtin_amdgcn_make_buffer_rsrc((void *)at, 0, left, 0x00020000);
+    }
+    __device__ __forceinline__ void advance() {   // behind the last K tile: loads of nothing keep the counts
+      --todo;
+      at += 128;
+      left = __builtin_amdgcn_readfirstlane(todo > 0 ? max(left - 128, 0) : 0);
+    }
   };
-  auto advance = [&]() { if (left > 1) { --left; koff += 128; } };   // past the end the last K tile is issued again
-  auto issue_scales = [&](int stage) { mx_dma16(sres, soff, spair, lds + MXT_SCALE + stage + wave * 1024); };
-  int sst = 0;   // scale stage of the current pair (byte offset)
-  auto advance_scales = [&]() { if (spairs > 1) { --spairs; spair += 16; } };
+  Stream w = {p.wc + (int64_t)n0 * cp + (int64_t)gbeg * 256, __builtin_amdgcn_readfirstlane(nr * cp - gbeg * 256), groups * 2};
+  Stream x = {p.xc + (int64_t)m0 * cp + (int64_t)gbeg * 256, __builtin_amdgcn_readfirstlane(mr * cp - gbeg * 256), groups * 2};
+  char *const dmaw = lds + wave * 8192;
+  auto issue = [&](const Stream &o, int q, int slot) { mx_dma16(o.rsrc(), voff[q], 0, dmaw + slot * MXT_OPER + q * 1024); };
+  const __amdgpu_buffer_rsrc_t wsr = mx_rsrc(p.ws, n0, nr, p.pitch), xsr = mx_rsrc(p.xs, m0, mr, p.pitch);
+  const unsigned soff = (unsigned)((wave * 64 + lane) * p.pitch);
+  unsigned sgrp = (unsigned)gbeg * 16;
+  const unsigned sgrp_last = (unsigned)(gbeg + groups - 1) * 16;
+  auto issue_scales = [&](int stage) {
+    mx_dma16(wsr, soff, sgrp, lds + MXT_SCALE + stage + wave * 1024);
+    mx_dma16(xsr, soff, sgrp, lds + MXT_SCALE + stage + 4096 + wave * 1024);
+    if (sgrp < sgrp_last) sgrp += 16;
+  };
 
+  // ---- fragments: weight rows (i >> 1) * 128 + wr * 64 + (i & 1) * 32 + fr, activation rows wc * 128 + j * 32 + fr
   const int fr = lane & 31, fh = lane >> 5;
   const int laneoff = fr * 128 + (((fh * 4) ^ (fr & 7)) << 4);
-  const char *ard[4], *brd[4];
+  const char *wrd[4], *xrd[4];
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
-    ard[s] = lds + ((wr * 64 * 128 + laneoff) ^ (s << 4));
-    brd[s] = lds + ((wc * 32 * 128 + laneoff) ^ (s << 4));
+    wrd[s] = lds + ((wr * 64 * 128 + laneoff) ^ (s << 4));
+    xrd[s] = lds + ((2 * MXT_OPER + wc * 128 * 128 + laneoff) ^ (s << 4));
   }
-  const char *asc = lds + MXT_SCALE + (wr * 64 + fr) * 16 + fh * 4, *bsc = lds + MXT_SCALE + (256 + wc * 32 + fr) * 16 + fh * 4;
+  // (the two scale pointers switch stages apart: activations are read one K tile ahead)
+  const char *wsc = lds + MXT_SCALE + (wr * 64 + fr) * 16 + fh * 4, *xsc = lds + MXT_SCALE + (256 + wc * 128 + fr) * 16 + fh * 4;
+  auto flip = [&](const char *q) { return (const char *)(lds + ((unsigned)(q - lds) ^ MXT_SCALE_STAGE)); };
 
-  f32x16 acc[4][2];
+  f32x16 acc[4][4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < 4; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
+  i32x4 a[2][4], b[2][4][4];     // [parity of i][step]; [K tile parity][j][step]
+  int as[2], bs[2][4];
+#define MX_READ_W(I, T, S) a[(I) & 1][S] = *(const i32x4 *)(wrd[S] + (T) * MXT_OPER + ((I) >> 1) * 16384 + ((I) & 1) * 4096);
+#define MX_SCALE_W(I, T) as[(I) & 1] = *(const int *)(wsc + ((I) >> 1) * 2048 + ((I) & 1) * 512 + (T) * 8);
+#define MX_READ_X(J, T, S) b[T][J][S] = *(const i32x4 *)(xrd[S] + (T) * MXT_OPER + (J) * 4096);
+#define MX_SCALE_X(J, T) bs[T][J] = *(const int *)(xsc + (J) * 512 + (T) * 8);
+#define MX_MMA(I, T, S, J) acc[I][J] = mx_mma(S, a[(I) & 1][S], b[T][J][S], acc[I][J], as[(I) & 1], bs[T][J]);
 
-  issue_scales(0); advance_scales();
+  issue_scales(0);
 #pragma unroll
-  for (int h = 0; h < 6; ++h) {
-    issue(h & 3, (h >> 2) & 1);
-    if ((h & 3) == 3) advance();
-  }
-  mx_wait<6>();
+  for (int q = 0; q < 8; ++q) issue(x, q, 2);
+#pragma unroll
+  for (int q = 0; q < 8; ++q) issue(w, q, 0);
+  x.advance(); w.advance();
+#pragma unroll
+  for (int q = 0; q < 8; ++q) issue(x, q, 3);
+  issue_scales(MXT_SCALE_STAGE);
+#pragma unroll
+  for (int q = 0; q < 8; ++q) issue(w, q, 1);
+  x.advance(); w.advance();
+  mx_wait<18>();
   __builtin_amdgcn_s_barrier();
-  if (wr == 1) __builtin_amdgcn_s_barrier();   // the second group runs one barrier behind
+#pragma unroll
+  for (int s = 0; s < 4; ++s) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { MX_READ_X(j, 0, s) }
+    MX_READ_W(0, 0, s)
+    MX_SCALE_X(s, 0)
+  }
+  MX_SCALE_W(0, 0)
 
-  i32x4 a[2][4], b[2][4];
-  int as[2], bs[2];
-#define MX_READ_A(ST, SLOT, HALF)                                                                       \
-  _Pragma("unroll") for (int s = 0; s < 4; ++s)                                                         \
-    _Pragma("unroll") for (int i = 0; i < 2; ++i)                                                       \
-      a[i][s] = *(const i32x4 *)(ard[s] + ST * MXT_STAGE + SLOT * MXT_HALF + i * 32 * 128);       \
-  _Pragma("unroll") for (int i = 0; i < 2; ++i)                                                         \
-    as[i] = *(const int *)(asc + (HALF * 128 + i * 32) * 16 + ST * 8);
-#define MX_READ_B(ST)                                                                                   \
-  _Pragma("unroll") for (int s = 0; s < 4; ++s)                                                         \
-    _Pragma("unroll") for (int j = 0; j < 2; ++j)                                                       \
-      b[j][s] = *(const i32x4 *)(brd[s] + ST * MXT_STAGE + (1 + j) * MXT_HALF);                   \
-  _Pragma("unroll") for (int j = 0; j < 2; ++j)                                                         \
-    bs[j] = *(const int *)(bsc + j * 128 * 16 + ST * 8);
-#define MX_STEP(AI, S)                                                                                  \
-  _Pragma("unroll") for (int i = 0; i < 2; ++i)                                                         \
-    _Pragma("unroll") for (int j = 0; j < 2; ++j)                                                       \
-      acc[AI + i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a[i][S]), wide(b[j][S]), acc[AI + i][j], 4, 4, S, as[i], S, bs[j]);
-#define MX_MFMAS(AI) MX_STEP(AI, 0) MX_STEP(AI, 1) MX_STEP(AI, 2) MX_STEP(AI, 3)
-#define MX_SYNC(N)                                                                                      \
-  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                                                    \
-  mx_wait<N>();                                                                                         \
-  __builtin_amdgcn_s_barrier();                                                                         \
-  __builtin_amdgcn_sched_barrier(0);                                                                    \
-  __builtin_amdgcn_s_setprio(1);
-#define MX_END                                                                                          \
-  __builtin_amdgcn_s_setprio(0);                                                                        \
-  __builtin_amdgcn_sched_barrier(0);                                                                    \
-  __builtin_amdgcn_s_barrier();
-// ST: K tile of the pair = code stage and half of the scale row; the first also issues the next pair's scales
-#define MX_KTILE(ST)                                                                                    \
-  {                                                                                                     \
-    MX_READ_A(ST, 0, 0) MX_READ_B(ST)                                                                   \
-    if constexpr (ST == 0) { issue_scales(sst ^ MXT_SCALE_STAGE); advance_scales(); }                   \
-    issue(2, 1 - ST); issue(3, 1 - ST); advance();                                                      \
-    MX_SYNC((ST ? 8 : 9))                                                                         \
-    MX_MFMAS(0)                                                                                         \
-    MX_END                                                                                              \
-    MX_READ_A(ST, 3, 1)                                                                                 \
-    issue(0, ST); issue(1, ST);                                                                 \
-    MX_SYNC(6)                                                                                          \
-    MX_MFMAS(2)                                                                                         \
-    MX_END                                                                                              \
+  // T: K tile of the group = stage of both operands.  x of K tile t + 1 is read from i = 1 on, w(i + 1) at i, w(0) of t + 1 at i = 3.
+  int sst = 0;         // scale stage of this group (bytes)
+#define MX_KTILE(T)                                                                                                 \
+  {                                                                                                                 \
+    _Pragma("unroll") for (int i = 0; i < 4; ++i) {                                                                 \
+      _Pragma("unroll") for (int y = 0; y < 16; ++y) {                                                              \
+        MX_MMA(i, T, y >> 2, y & 3)                                                                                 \
+        if (i < 3) {                                                                                                \
+          if (y < 4) { MX_READ_W(i + 1, T, y) }                                                                     \
+          if (y == 4) { MX_SCALE_W(i + 1, T) }                                                                      \
+        }                                                                                                           \
+        if (i == 0 && y == 12) {              /* x of t + 1 has landed; every wave has left x of t */               \
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                                                        \
+          mx_wait<(T) ? 8 : 10>();                                                                                  \
+          __builtin_amdgcn_s_barrier();                                                                             \
+          if constexpr ((T) == 1) xsc = flip(xsc);                                                                  \
+        }                                                                                                           \
+        if (i == 1 && y >= 8) issue(x, y - 8, 2 + (T));                                                             \
+        if (i == 1 && y >= 8 && y < 12) { MX_READ_X(0, 1 - (T), y - 8) }                                            \
+        if (i == 1 && y >= 12) { MX_SCALE_X(y - 12, 1 - (T)) }                                                      \
+        if (i == 2 && y >= 6 && y < 14) { MX_READ_X(1 + ((y - 6) >> 2), 1 - (T), (y - 6) & 3) }                     \
+        if (i == 3 && y == 2) {               /* w of t + 1 has landed; every wave has left w of t */               \
+          asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");                                                        \
+          mx_wait<8>();                                                                                             \
+          __builtin_amdgcn_s_barrier();                                                                             \
+          if constexpr ((T) == 1) { wsc = flip(wsc); issue_scales(sst); }                                           \
+        }                                                                                                           \
+        if (i == 3 && y >= 3 && y < 7) { MX_READ_W(0, 1 - (T), y - 3) }                                             \
+        if (i == 3 && y == 7) { MX_SCALE_W(0, 1 - (T)) }                                                            \
+        if (i == 3 && y >= 4 && y < 12) issue(w, y - 4, T);                                                         \
+        if (i == 3 && y >= 8 && y < 12) { MX_READ_X(3, 1 - (T), y - 8) }                                            \
+        __builtin_amdgcn_sched_barrier(0);                                                                          \
+      }                                                                                                             \
+    }                                                                                                               \
+    x.advance(); w.advance();                                                                                       \
   }
-  for (int k = 0; k < pairs; ++k) {
+  for (int g = 0; g < groups; ++g) {
     MX_KTILE(0)
     MX_KTILE(1)
     sst ^= MXT_SCALE_STAGE;
-    asc = lds + ((unsigned)(asc - lds) ^ MXT_SCALE_STAGE);
-    bsc = lds + ((unsigned)(bsc - lds) ^ MXT_SCALE_STAGE);
   }
 #undef MX_KTILE
-#undef MX_END
-#undef MX_SYNC
-#undef MX_MFMAS
-#undef MX_STEP
-#undef MX_READ_B
-#undef MX_READ_A
-  if (wr == 0) __builtin_amdgcn_s_barrier();
+#undef MX_MMA
+#undef MX_SCALE_X
+#undef MX_READ_X
+#undef MX_SCALE_W
+#undef MX_READ_W
   mx_wait<0>();        // the tail loads must have landed before the stages are reused
   __syncthreads();
 
@@ -459,40 +490,45 @@ template <typename TO> __global__ __launch_bounds__(512, 2) void mx_dense256_ker
   const bool raw = p.split > 1;
   TO *const y = raw ? (TO *)p.slab + (int64_t)sk * p.M * p.N : (TO *)p.y;
   const int64_t ldy = raw ? p.N : p.ldy;
-#pragma unroll
-  for (int h = 0; h < NPASS; ++h) {
-    if (h) __syncthreads();
+  const bool sig = p.act == CFD_ACT_SIGMOID && !raw;
+  const float ns = raw || sig ? 1.f : act_neg_scale(p.act, p.slope);
+  float *const sbias = (float *)(lds + 256 * MXT_ROW);
+  sbias[tid] = p.bias && !raw && n0 + tid < p.N ? p.bias[n0 + tid] : 0.f;
+  __syncthreads();
+  auto to_lds = [&](int h, auto with_sigmoid) {   // two copies, chosen once: 256 elements a lane
 #pragma unroll
     for (int ii = 0; ii < 4 / NPASS; ++ii) {
       const int i = h * 2 + ii;
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const int nl = (i >> 1) * 128 + wr * 64 + (i & 1) * 32 + q * 8 + fh * 4;
-        f32x4 bv = {0.f, 0.f, 0.f, 0.f};
-        if (p.bias && !raw) {
+        const f32x4 bv = *(const f32x4 *)(sbias + nl);
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (n0 + nl + r < p.N) bv[r] = p.bias[n0 + nl + r];
-        }
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
+        for (int j = 0; j < 4; ++j) {
           TO o[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float v = acc[i][j][q * 4 + r] + bv[r];
-            o[r] = (TO)(raw ? v : apply_act(v, p.act, p.slope));
+            float v = acc[i][j][q * 4 + r] + bv[r];
+            if constexpr (decltype(with_sigmoid)::value) v = 1.f / (1.f + __expf(-v));
+            o[r] = (TO)apply_act_linear(v, ns);
           }
-          char *d = lds + (j * 128 + wc * 32 + fr) * MXT_ROW + (nl - h * COLS) * ES;
+          char *d = lds + (wc * 128 + j * 32 + fr) * MXT_ROW + (nl - h * COLS) * ES;
           if constexpr (ES == 2) *(bf16x4 *)d = (bf16x4){o[0], o[1], o[2], o[3]};
           else *(f32x4 *)d = (f32x4){o[0], o[1], o[2], o[3]};
         }
       }
     }
+  };
+#pragma unroll
+  for (int h = 0; h < NPASS; ++h) {
+    if (h) __syncthreads();
+    if (sig) to_lds(h, std::true_type{});
+    else to_lds(h, std::false_type{});
     __syncthreads();
     const int c = (lane & 31) * EPC, n = n0 + h * COLS + c;
 #pragma unroll 4
-    for (int it = 0; it < 16; ++it) {
-      const int ml = wave * 32 + it * 2 + (lane >> 5);
+    for (int it = 0; it < 32; ++it) {
+      const int ml = wave * 64 + it * 2 + (lane >> 5);
       if (ml >= mr || n >= p.N) continue;
       const char *src = lds + ml * MXT_ROW + c * ES;
       TO *dst = y + (int64_t)(m0 + ml) * ldy + n;
@@ -619,11 +655,11 @@ static void mx_plan(MxDense &p, bool serve) {
   if (p.big) {
     p.nt = (p.N + 255) / 256;
     p.mt = (p.M + 255) / 256;
-    const int groups = (p.nb + 7) / 8;
+    const int groups = p.pitch / 16;
     int64_t want = 256 / ((int64_t)p.nt * p.mt);
-    if (want > groups / 8) want = groups / 8;
+    if (want > groups / 4) want = groups / 4;
     if (want < 1) want = 1;
-    p.kt_per = (int)(((groups + want - 1) / want + 1) / 2 * 2);   // whole pairs of K tiles
+    p.kt_per = (int)((groups + want - 1) / want);
     p.split = (groups + p.kt_per - 1) / p.kt_per;
     return;
   }
@@ -728,8 +764,8 @@ extern "C" int cfd_mxfp4_dense(const cfd_mxfp4_dense_desc *d, const void *x, con
     const bool b16 = p.out_bf16 && p.split == 1;
     const void *fn = b16 ? (const void *)mx_dense256_kernel<bf16> : (const void *)mx_dense256_kernel<float>;
     if (int rc = set_max_lds(fn, MXT_LDS)) return rc;
-    if (b16) hipLaunchKernelGGL(mx_dense256_kernel<bf16>, dim3((unsigned)blocks), dim3(512), MXT_LDS, st, p);
-    else hipLaunchKernelGGL(mx_dense256_kernel<float>, dim3((unsigned)blocks), dim3(512), MXT_LDS, st, p);
+    if (b16) hipLaunchKernelGGL(mx_dense256_kernel<bf16>, dim3((unsigned)blocks), dim3(256), MXT_LDS, st, p);
+    else hipLaunchKernelGGL(mx_dense256_kernel<float>, dim3((unsigned)blocks), dim3(256), MXT_LDS, st, p);
   } else if (d->x_kind == CFD_MX_X_MXFP4) hipLaunchKernelGGL(mx_dense_kernel, dim3((unsigned)blocks), dim3(256), 0, st, p);
   else if (d->x_kind == CFD_MX_X_BF16) hipLaunchKernelGGL(mx_serve_kernel<bf16>, dim3((unsigned)blocks), dim3(256), 0, st, p);
   else hipLaunchKernelGGL(mx_serve_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, st, p);
