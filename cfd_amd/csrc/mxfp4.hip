@@ -198,6 +198,8 @@ struct MxDense {
   int mt, nt;
   int out_bf16, act;
   float slope;
+  int kwaves;                         // float activations: waves of a workgroup that share a weight tile
+  int xrows;                          //   and activation rows of a tile (<= 16)
   bool big;                           // 256 x 256 tiles
 };
 
@@ -220,15 +222,34 @@ __device__ __forceinline__ void mx_emit(const MxDense &p, int sk, int64_t m, int
     if (n + r < p.N) mx_store(p, m, n + r, apply_act(v[r] + (p.bias ? p.bias[n + r] : 0.f), p.act, p.slope));
 }
 
-// sums of the split slabs in a fixed order, bias, activation, output type
+// sums of the split slabs, bias, activation, output type: 16 lanes take 64 consecutive outputs, 16 groups of lanes take the
+// slabs in turn (every load of a thread in flight at once: one thread per output and a loop over 128 slabs took 31 us for
+// 256 outputs) and join in LDS.  The order is fixed: same inputs, same bits.
 __global__ __launch_bounds__(256) void mx_split_sum_kernel(MxDense p) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, MN = (int64_t)p.M * p.N;
-  if (i >= MN) return;
-  float s = 0.f;
-  for (int k = 0; k < p.split; ++k) s += p.slab[k * MN + i];
-  const int64_t m = i / p.N;
-  const int n = (int)(i - m * p.N);
-  mx_store(p, m, n, apply_act(s + (p.bias ? p.bias[n] : 0.f), p.act, p.slope));
+  __shared__ f32x4 part[16][16];
+  const int l = threadIdx.x & 15, g = threadIdx.x >> 4;
+  const int64_t MN = (int64_t)p.M * p.N, i = (int64_t)blockIdx.x * 64 + l * 4;
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  if (i + 4 <= MN) {
+#pragma unroll 8
+    for (int k = g; k < p.split; k += 16) s += *(const f32x4a4 *)(p.slab + k * MN + i);
+  } else {
+    for (int k = g; k < p.split; k += 16)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (i + e < MN) s[e] += p.slab[k * MN + i + e];
+  }
+  part[g][l] = s;
+  __syncthreads();
+  if (g >= 4) return;
+  const int64_t o = (int64_t)blockIdx.x * 64 + threadIdx.x;   // one output a thread
+  if (o >= MN) return;
+  float v = 0.f;
+#pragma unroll
+  for (int k = 0; k < 16; ++k) v += part[k][threadIdx.x >> 2][threadIdx.x & 3];
+  const int64_t m = o / p.N;
+  const int n = (int)(o - m * p.N);
+  mx_store(p, m, n, apply_act(v + (p.bias ? p.bias[n] : 0.f), p.act, p.slope));
 }
 
 constexpr unsigned MX_OOB = 0x80000000u;
@@ -241,51 +262,78 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_rsrc(const uint8_t *base, i
   return __builtin_amdgcn_make_buffer_rsrc((void *)(base + row0 * pitch), 0, (int)(rows * pitch), 0x00020000);
 }
 
-// Both operands in 4 bits, any shape: a workgroup of four waves owns 64 (m) x 64 (n), a wave 32 x 32, fragments go from
-// global memory straight into the scaled MFMA (16x16x128: lane = row l & 15, block l >> 4; its scale byte is the lane's own).
-// A K group is 256 columns = two MFMA steps; lane group g takes the blocks 2g and 2g + 1 of the group, so one 16-bit load
-// holds both of its scales and the step picks the byte.
-__global__ __launch_bounds__(256) void mx_dense_kernel(MxDense p) {
-  int bid = blockIdx.x;
-  const int nt = bid % p.nt; bid /= p.nt;
-  const int mt = bid % p.mt;
-  const int sk = bid / p.mt;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
-  const int m0 = mt * 64, n0 = nt * 64;
-  const int cp = p.nb * 16;
+// tile of a workgroup: each XCD (it has its own L2) gets a contiguous run of them; the tiles of one K slice follow each other
+__device__ __forceinline__ void mx_small_tile(const MxDense &p, int &mt, int &nt, int &sk) {
+  const int nwg = p.mt * p.nt * p.split, q = nwg >> 3, r = nwg & 7, xcd = blockIdx.x & 7;
+  int t = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + ((int)blockIdx.x >> 3);
+  mt = t % p.mt; t /= p.mt;
+  nt = t % p.nt;
+  sk = __builtin_amdgcn_readfirstlane(t / p.nt);
+  mt = __builtin_amdgcn_readfirstlane(mt);
+  nt = __builtin_amdgcn_readfirstlane(nt);
+}
+
+// Both operands in 4 bits, small or long products (bound by reading them): a workgroup owns 64 (m) x 64 (n), its four waves take
+// K groups of 256 columns in turn and join in LDS.  Fragments go from global memory straight into the scaled MFMA
+// (16x16x128: lane = row l & 15, block l >> 4, its scale byte its own); lane group g takes blocks 2g and 2g + 1 of a K
+// group, so one 16-bit load holds both of its scales and the step picks the byte.  A wave loads two K groups at a time.
+// Codes behind the last column (the next row's) need no mask: their scale bytes are zero on both operands, 2^-254 is zero in fp32.
+__global__ __launch_bounds__(256, 2) void mx_dense_kernel(MxDense p) {
+  __shared__ f32x4 part[4][16][64];
+  int mt, nt, sk;
+  mx_small_tile(p, mt, nt, sk);
+  const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int m0 = mt * 64, n0 = nt * 64, cp = p.nb * 16;
   const int mr = min(64, p.M - m0), nr = min(64, p.N - n0);
   const __amdgpu_buffer_rsrc_t xr = mx_rsrc(p.xc, m0, mr, cp), wr = mx_rsrc(p.wc, n0, nr, cp);
   const __amdgpu_buffer_rsrc_t xsr = mx_rsrc(p.xs, m0, mr, p.pitch), wsr = mx_rsrc(p.ws, n0, nr, p.pitch);
-  const int wm = (wave & 1) * 32, wn = (wave >> 1) * 32;
-  f32x4 acc[2][2] = {};
-  const int k0 = sk * p.kt_per, k1 = min(k0 + p.kt_per, (p.nb + 7) / 8);
-  for (int kt = k0; kt < k1; ++kt) {
+  f32x4 acc[4][4] = {};
+  struct Group { i32x4 a[4][2], b[4][2]; int as[4], bs[4]; };
+  auto load = [&](Group &g, int kt) {
     const int b0 = kt * 8 + fq * 2;
-    i32x4 a[2][2], b[2][2];
-    int as[2], bs[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int rw = wn + i * 16 + fr, rx = wm + i * 16 + fr;
+    for (int i = 0; i < 4; ++i) {
+      // rows past the operand lie past its size and read as zero; kt < 0: nothing left to load
+      const unsigned row = (unsigned)(i * 16 + fr), co = kt < 0 ? MX_OOB : row * cp + b0 * 16, so = kt < 0 ? MX_OOB : row * p.pitch + b0;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        a[i][s] = ld16(wr, b0 + s < p.nb && rw < nr ? (unsigned)(rw * cp + (b0 + s) * 16) : MX_OOB);
-        b[i][s] = ld16(xr, b0 + s < p.nb && rx < mr ? (unsigned)(rx * cp + (b0 + s) * 16) : MX_OOB);
+        g.a[i][s] = ld16(wr, co + s * 16);
+        g.b[i][s] = ld16(xr, co + s * 16);
       }
-      as[i] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(wsr, rw < nr ? (int)(rw * p.pitch + b0) : (int)MX_OOB, 0, 0);
-      bs[i] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(xsr, rx < mr ? (int)(rx * p.pitch + b0) : (int)MX_OOB, 0, 0);
+      g.as[i] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(wsr, (int)so, 0, 0);
+      g.bs[i] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(xsr, (int)so, 0, 0);
     }
+  };
+  auto multiply = [&](const Group &g) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(a[i][0]), wide(b[j][0]), acc[i][j], 4, 4, 0, as[i], 0, bs[j]);
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(a[i][1]), wide(b[j][1]), acc[i][j], 4, 4, 1, as[i], 1, bs[j]);
+      for (int j = 0; j < 4; ++j) {
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(g.a[i][0]), wide(g.b[j][0]), acc[i][j], 4, 4, 0, g.as[i], 0, g.bs[j]);
+        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(g.a[i][1]), wide(g.b[j][1]), acc[i][j], 4, 4, 1, g.as[i], 1, g.bs[j]);
       }
+  };
+  const int k1 = min((sk + 1) * p.kt_per, (p.nb + 7) / 8);
+  for (int kt = sk * p.kt_per + wave; kt < k1; kt += 8) {
+    Group g0, g1;
+    load(g0, kt);
+    load(g1, kt + 4 < k1 ? kt + 4 : -1);
+    multiply(g0);
+    multiply(g1);
   }
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) mx_emit(p, sk, m0 + wm + j * 16 + fr, n0 + wn + i * 16 + fq * 4, acc[i][j]);
+    for (int j = 0; j < 4; ++j) part[wave][i * 4 + j][lane] = acc[i][j];
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {     // wave i sums weight rows i * 16 .. + 15
+    f32x4 t = part[0][wave * 4 + j][lane];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) t += part[w][wave * 4 + j][lane];
+    mx_emit(p, sk, m0 + j * 16 + fr, n0 + wave * 16 + fq * 4, t);
+  }
 }
 
 // Large products: 256 (n) x 256 (m) tile, four waves of 128 x 128 (one per SIMD, 256 accumulators in the accumulation
@@ -539,12 +587,13 @@ template <typename TO> __global__ __launch_bounds__(256, 1) void mx_dense256_ker
   }
 }
 
-// Float activations against 4-bit weights (serving: the weights are what is read).  A wave owns 64 weight rows x 16
-// activation rows; a K group is 512 columns: lane group g takes blocks 4g..4g+3, so a lane reads 64 contiguous bytes of
-// codes and one 32-bit word of scales.  Codes become bf16 with their scale applied (exact: two significant bits) and meet
-// the activations in 16x16x32 bf16 MFMAs, whose k order is the lane's block order on both operands.  fp32 activations are
-// split exactly into three bf16 terms (8 + 8 + 8 bits by truncation) and take three MFMAs: fp32 accuracy, the weights
-// are still read once.  The four waves of a workgroup take K groups in turn and join in LDS.
+// Float activations against 4-bit weights (serving: the weights are what is read).  A workgroup's four waves own 64 weight rows
+// each (or, where the layer is narrower, share the K groups) x 16 activation rows.  A K group is 512 columns: lane group g takes
+// blocks 4g..4g+3, so a lane reads 64 contiguous bytes of codes and one 32-bit word of scales.  Codes become bf16 with
+// their scale applied (exact: two significant bits) and meet the activations in 16x16x32 bf16 MFMAs, whose k order is the
+// lane's block order on both operands.  The activations of a K group are converted once per workgroup and wait in LDS; fp32 ones
+// are split exactly into three bf16 terms (8 + 8 + 8 bits by truncation) and take three MFMAs: fp32 accuracy, the weights are
+// still read once.
 struct Split3 { bf16 t[3]; };
 __device__ __forceinline__ Split3 split3(float x) {
   Split3 r;
@@ -564,31 +613,59 @@ __device__ __forceinline__ bf16x8 mx_bf16x8(unsigned c, float s) {
   return (bf16x8){a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1]};
 }
 
+constexpr int MXS_ROW = 1024 + 16;      // bytes of one activation row's K group in LDS: 512 bf16 and a pad
 template <typename TX> __global__ __launch_bounds__(256) void mx_serve_kernel(MxDense p) {
   constexpr int NX = sizeof(TX) == 4 ? 3 : 1;
-  __shared__ f32x4 part[4][4][64];
-  int bid = blockIdx.x;
-  const int nt = bid % p.nt; bid /= p.nt;
-  const int mt = bid % p.mt;
-  const int sk = bid / p.mt;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, fr = lane & 15, fq = lane >> 4;
-  const int m = mt * 16 + fr, n0 = nt * 64;
-  const int cp = p.nb * 16, nr = min(64, p.N - n0);
-  const __amdgpu_buffer_rsrc_t wr = mx_rsrc(p.wc, n0, nr, cp), wsr = mx_rsrc(p.ws, n0, nr, p.pitch);
-  const TX *x = (const TX *)p.x + (int64_t)m * p.ldx;
+  extern __shared__ __attribute__((aligned(16))) char lds[];    // [K groups of a round][NX][rows], then the partial sums
+  int mt, nt, sk;
+  mx_small_tile(p, mt, nt, sk);
+  const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kw = p.kwaves, wk = wave % kw, wn = wave / kw;       // K groups taken at once; this wave's group and weight rows
+  const int m0 = mt * 16, n0 = (nt * (4 / kw) + wn) * 64;
+  const int cp = p.nb * 16, nr = max(0, min(64, p.N - n0)), rows = min(16, p.M - m0);
+  const __amdgpu_buffer_rsrc_t wr = mx_rsrc(p.wc, nr ? n0 : 0, nr, cp), wsr = mx_rsrc(p.ws, nr ? n0 : 0, nr, p.pitch);
   f32x4 acc[4] = {};
   const int k0 = sk * p.kt_per, k1 = min(k0 + p.kt_per, (p.nb + 15) / 16);
-  for (int kt = k0 + wave; kt < k1; kt += 4) {
-    const int b0 = kt * 16 + fq * 4;
+  const int gbytes = NX * p.xrows * MXS_ROW;
+  for (int kt = k0; kt < k1; kt += kw) {
+    // this wave's codes are on their way while the workgroup converts the activations
+    const int b0 = (kt + wk) * 16 + fq * 4;
+    const bool mine = kt + wk < k1;
     i32x4 c[4][4];
     unsigned sc[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int r = i * 16 + fr;
-      sc[i] = (unsigned)__builtin_amdgcn_raw_buffer_load_b32(wsr, r < nr ? (int)(r * p.pitch + b0) : (int)MX_OOB, 0, 0);
+      const unsigned r = (unsigned)(i * 16 + fr);
+      sc[i] = (unsigned)__builtin_amdgcn_raw_buffer_load_b32(wsr, mine ? (int)(r * p.pitch + b0) : (int)MX_OOB, 0, 0);
 #pragma unroll
-      for (int s = 0; s < 4; ++s) c[i][s] = ld16(wr, b0 + s < p.nb && r < nr ? (unsigned)(r * cp + (b0 + s) * 16) : MX_OOB);
+      for (int s = 0; s < 4; ++s) c[i][s] = ld16(wr, mine ? r * cp + b0 * 16 + s * 16 : MX_OOB);   // (behind K: times zero)
     }
+    if (kt > k0) __syncthreads();
+    // 8 columns a thread: 64 threads a row and K group
+    const int items = min(kw, k1 - kt) * p.xrows;
+    for (int t = wave; t < items; t += 4) {
+      const int col = lane * 8, g = t / p.xrows, row = t - g * p.xrows;
+      const int k = (kt + g) * 512 + col;
+      float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (row < rows && k < p.K) load8((const TX *)p.x + (int64_t)(m0 + row) * p.ldx + k, p.K - k, v);
+      bf16x8 o[NX];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (NX == 1) o[0][e] = (bf16)v[e];
+        else {
+          const Split3 q = split3(v[e]);
+#pragma unroll
+          for (int u = 0; u < 3; ++u) o[u][e] = q.t[u];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < NX; ++u) *(bf16x8 *)(lds + g * gbytes + (u * p.xrows + row) * MXS_ROW + col * 2) = o[u];
+    }
+    __syncthreads();
+    if (!mine) continue;      // (uniform; no weights, and zero times an infinite activation is not zero)
+    // (lanes past the rows there are read row 0: a column of the product that nobody stores)
+    const char *xl = lds + wk * gbytes + (fr < p.xrows ? fr : 0) * MXS_ROW + fq * 256;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       float sf[4];
@@ -599,39 +676,31 @@ template <typename TX> __global__ __launch_bounds__(256) void mx_serve_kernel(Mx
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const int k = (b0 + s) * 32 + j * 8;
-        float v[8];
-        if (m < p.M && k < p.K) load8(x + k, p.K - k, v);
-        else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] = 0.f;
-        }
         bf16x8 xb[NX];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if constexpr (NX == 1) xb[0][e] = (bf16)v[e];
-          else {
-            const Split3 q = split3(v[e]);
-#pragma unroll
-            for (int t = 0; t < 3; ++t) xb[t][e] = q.t[t];
-          }
-        }
+        for (int u = 0; u < NX; ++u) xb[u] = *(const bf16x8 *)(xl + u * p.xrows * MXS_ROW + s * 64 + j * 16);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const bf16x8 wv = mx_bf16x8((unsigned)c[i][s][j], sf[i]);
 #pragma unroll
-          for (int t = NX - 1; t >= 0; --t) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xb[t], acc[i], 0, 0, 0);
+          for (int u = NX - 1; u >= 0; --u) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xb[u], acc[i], 0, 0, 0);
         }
       }
     }
   }
+  if (kw > 1) {          // the waves of one weight tile join
+    __syncthreads();
+    f32x4 *part = (f32x4 *)lds;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) part[wave][i][lane] = acc[i];
-  __syncthreads();
-  f32x4 t = part[0][wave][lane];
+    for (int i = 0; i < 4; ++i) part[(wave * 4 + i) * 64 + lane] = acc[i];
+    __syncthreads();
+    if (wk) return;
 #pragma unroll
-  for (int w = 1; w < 4; ++w) t += part[w][wave][lane];
-  mx_emit(p, sk, m, n0 + wave * 16 + fq * 4, t);
+    for (int i = 0; i < 4; ++i)
+      for (int w = 1; w < kw; ++w) acc[i] += part[((wave + w) * 4 + i) * 64 + lane];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) mx_emit(p, sk, m0 + fr, n0 + i * 16 + fq * 4, acc[i]);
 }
 
 static int mx_check(int64_t m, int64_t n, int64_t k) {
@@ -640,32 +709,43 @@ static int mx_check(int64_t m, int64_t n, int64_t k) {
   return CFD_OK;
 }
 
-// K slices: enough workgroups to fill the chip (4 per CU), no slice under `least` groups
-static void mx_split(MxDense &p, int groups, int64_t tiles, int least) {
-  int64_t want = 1024 / tiles;
-  if (want > groups / least) want = groups / least;
+static void mx_split(MxDense &p, int groups, int64_t want) {   // K slices of whole groups, about `want` of them
+  if (want > groups) want = groups;
   if (want < 1) want = 1;
   p.kt_per = (int)((groups + want - 1) / want);
   p.split = (groups + p.kt_per - 1) / p.kt_per;
 }
-static void mx_plan(MxDense &p, bool serve) {
+static int mx_serve_bytes(const MxDense &p, int x_kind) {   // LDS of the float-activation kernel
+  const int groups = p.kt_per < p.kwaves ? p.kt_per : p.kwaves;
+  const int x = groups * (x_kind == CFD_MX_X_BF16 ? 1 : 3) * p.xrows * MXS_ROW, sums = p.kwaves > 1 ? 4 * 4 * 64 * 16 : 0;
+  return x > sums ? x : sums;
+}
+static void mx_plan(MxDense &p, int x_kind) {
+  const bool serve = x_kind != CFD_MX_X_MXFP4;
   p.nb = (int)mx_blocks(p.K);
   p.pitch = (int)mx_scale_pitch(p.K);
   p.big = !serve && p.M > 128 && p.N > 128;
   if (p.big) {
     p.nt = (p.N + 255) / 256;
     p.mt = (p.M + 255) / 256;
-    const int groups = p.pitch / 16;
-    int64_t want = 256 / ((int64_t)p.nt * p.mt);
-    if (want > groups / 4) want = groups / 4;
-    if (want < 1) want = 1;
-    p.kt_per = (int)((groups + want - 1) / want);
-    p.split = (groups + p.kt_per - 1) / p.kt_per;
-    return;
+    const int groups = p.pitch / 16;     // one workgroup per CU; a slice has 4 groups at least
+    const int64_t want = 256 / ((int64_t)p.nt * p.mt);
+    mx_split(p, groups, want < groups / 4 ? want : groups / 4);
+  } else if (serve) {
+    p.mt = (p.M + 15) / 16;
+    p.xrows = p.M < 16 ? p.M : 16;
+    for (p.kwaves = p.N <= 64 ? 4 : p.N <= 128 ? 2 : 1;; p.kwaves /= 2) {   // (fewer where their activations exceed the LDS)
+      p.nt = (p.N + 256 / p.kwaves - 1) / (256 / p.kwaves);
+      mx_split(p, (p.nb + 15) / 16, 512 / ((int64_t)p.nt * p.mt));
+      if (p.kwaves == 1 || mx_serve_bytes(p, x_kind) <= 128 * 1024) break;
+    }
+  } else {
+    p.nt = (p.N + 63) / 64;
+    p.mt = (p.M + 63) / 64;
+    const int groups = (p.nb + 7) / 8;   // two workgroups per CU; a slice has a group for each of the four waves
+    const int64_t want = 512 / ((int64_t)p.nt * p.mt);
+    mx_split(p, groups, want < groups / 4 ? want : groups / 4);
   }
-  p.nt = (p.N + 63) / 64;
-  p.mt = serve ? (p.M + 15) / 16 : (p.M + 63) / 64;
-  mx_split(p, serve ? (p.nb + 15) / 16 : (p.nb + 7) / 8, (int64_t)p.nt * p.mt, 4);
 }
 
 }  // namespace cfd
@@ -728,12 +808,13 @@ extern "C" int cfd_mxfp4_dequantize(const uint8_t *codes, const uint8_t *scales,
   return CFD_OK;
 }
 
-extern "C" int64_t cfd_mxfp4_dense_workspace_bytes(int64_t m, int64_t n, int64_t k, int x_float) {
+extern "C" int64_t cfd_mxfp4_dense_workspace_bytes(int64_t m, int64_t n, int64_t k, int x_kind) {
   if (int rc = mx_check(m, n, k)) return rc;
+  CFD_REQUIRE(x_kind >= CFD_MX_X_F32 && x_kind <= CFD_MX_X_MXFP4, "bad x_kind");
   if (!m || !n) return 0;
   MxDense p = {};
   p.M = (int)m; p.N = (int)n; p.K = (int)k;
-  mx_plan(p, x_float != 0);
+  mx_plan(p, x_kind);
   return p.split > 1 ? (int64_t)p.split * m * n * 4 : 0;
 }
 
@@ -752,7 +833,7 @@ extern "C" int cfd_mxfp4_dense(const cfd_mxfp4_dense_desc *d, const void *x, con
   CFD_REQUIRE(serve || (((uintptr_t)x | (uintptr_t)x_scales) & 15) == 0, "4-bit activations must be 16-byte aligned");
   MxDense p = {};
   p.M = (int)d->m; p.N = (int)d->n; p.K = (int)d->k;
-  mx_plan(p, serve);
+  mx_plan(p, d->x_kind);
   p.xc = (const uint8_t *)x; p.xs = x_scales; p.x = x; p.ldx = d->ldx; p.wc = w_codes; p.ws = w_scales; p.bias = bias;
   p.y = y; p.ldy = d->ldy; p.out_bf16 = d->out_dtype == CFD_BF16; p.act = d->act; p.slope = d->leaky_slope;
   p.slab = (float *)ws;
@@ -766,12 +847,21 @@ extern "C" int cfd_mxfp4_dense(const cfd_mxfp4_dense_desc *d, const void *x, con
     if (int rc = set_max_lds(fn, MXT_LDS)) return rc;
     if (b16) hipLaunchKernelGGL(mx_dense256_kernel<bf16>, dim3((unsigned)blocks), dim3(256), MXT_LDS, st, p);
     else hipLaunchKernelGGL(mx_dense256_kernel<float>, dim3((unsigned)blocks), dim3(256), MXT_LDS, st, p);
-  } else if (d->x_kind == CFD_MX_X_MXFP4) hipLaunchKernelGGL(mx_dense_kernel, dim3((unsigned)blocks), dim3(256), 0, st, p);
-  else if (d->x_kind == CFD_MX_X_BF16) hipLaunchKernelGGL(mx_serve_kernel<bf16>, dim3((unsigned)blocks), dim3(256), 0, st, p);
-  else hipLaunchKernelGGL(mx_serve_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, st, p);
+  } else if (!serve) {
+    hipLaunchKernelGGL(mx_dense_kernel, dim3((unsigned)blocks), dim3(256), 0, st, p);
+  } else {
+    const bool b16 = d->x_kind == CFD_MX_X_BF16;
+    const int bytes = mx_serve_bytes(p, d->x_kind);
+    const void *fn = b16 ? (const void *)mx_serve_kernel<bf16> : (const void *)mx_serve_kernel<float>;
+    if (bytes > 64 * 1024)
+      if (int rc = set_max_lds(fn, bytes)) return rc;
+    if (b16) hipLaunchKernelGGL(mx_serve_kernel<bf16>, dim3((unsigned)blocks), dim3(256), bytes, st, p);
+    else hipLaunchKernelGGL(mx_serve_kernel<float>, dim3((unsigned)blocks), dim3(256), bytes, st, p);
+  }
   CFD_LAUNCH_CHECK();
   if (p.split > 1) {
-    const int64_t b = (d->m * d->n + 255) / 256;
+    const int64_t b = (d->m * d->n + 63) / 64;
+    CFD_REQUIRE(b <= 0x7fffffff, "too many outputs");
     hipLaunchKernelGGL(mx_split_sum_kernel, dim3((unsigned)b), dim3(256), 0, st, p);
     CFD_LAUNCH_CHECK();
   }

@@ -1104,7 +1104,7 @@ def mxfp4_dense(x: Union[Mxfp4, torch.Tensor], w: Mxfp4, bias: Optional[torch.Te
             return out
         d = Mxfp4DenseDesc(x_kind=kind, out_dtype=_DT[odt], act=act, leaky_slope=slope, m=m, n=n, k=k, ldx=ldx,
                            ldy=_mx_input(out, "mxfp4_dense: out"))
-        wsb = lib.cfd_mxfp4_dense_workspace_bytes(m, n, k, int(not four))
+        wsb = lib.cfd_mxfp4_dense_workspace_bytes(m, n, k, kind)
         if wsb < 0:
             check(-1, "cfd_mxfp4_dense_workspace_bytes")
         ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None

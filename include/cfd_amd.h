@@ -378,7 +378,7 @@ typedef struct {
   float leaky_slope;
   int64_t m, n, k, ldx, ldy;
 } cfd_mxfp4_dense_desc;
-int64_t cfd_mxfp4_dense_workspace_bytes(int64_t m, int64_t n, int64_t k, int x_float);
+int64_t cfd_mxfp4_dense_workspace_bytes(int64_t m, int64_t n, int64_t k, int x_kind);
 int cfd_mxfp4_dense(const cfd_mxfp4_dense_desc *desc, const void *x, const uint8_t *x_scales, const uint8_t *w_codes,
                     const uint8_t *w_scales, const float *bias, void *y, void *ws, void *stream);
 
