@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes as C
+from array import array
 from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import numpy as np
@@ -918,22 +919,33 @@ def conv_first_wgrad(x, x2, dpre, dw, db, ksize, stride):
 # ----------------------------------------------------------------------------------------
 # optimizer over a list of tensors (trainer.AdamW keeps the state)
 # ----------------------------------------------------------------------------------------
-def _on(device: torch.device):
+def _on(index: int):
     """launches go to the tensors' device and its current stream, whatever device is current"""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return contextlib.nullcontext() if index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
-def _tensor_list(ts: Sequence[torch.Tensor], what: str, dtype: Optional[torch.dtype] = None,
-                 device: Optional[torch.device] = None) -> None:
-    """dense device tensors of one dtype (fp32 or bf16) on one device"""
+def _raw_stream(index: int) -> int:
+    """the handle of the device's current stream (a tenth of what building a torch.cuda.Stream for it costs)"""
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
+_T = torch.Tensor
+
+
+def _tensor_list(ts: Sequence[torch.Tensor], what: str, dtype: Optional[torch.dtype] = None, device: Optional[int] = None) -> None:
+    """dense device tensors of one dtype (fp32 or bf16) on one device; checked by whole-list calls, which cost a tenth of a
+    microsecond a tensor"""
+    dtypes, devices = {t.dtype for t in ts}, set(map(_T.get_device, ts))
+    if len(dtypes) <= 1 and len(devices) <= 1 and -1 not in devices and (dtype is None or dtypes <= {dtype}) and dtypes <= _DT.keys() \
+            and (device is None or devices <= {device}) and all(map(_T.is_contiguous, ts)):
+        return
     for t in ts:
-        dtype, device = dtype or t.dtype, device or t.device
-        if not t.is_cuda or t.dtype != dtype or t.device != device or not t.is_contiguous():
-            _dev(t)
-            _need(t.device == device, f"{what} on {t.device}, the others on {device}")
-            _need(t.dtype == dtype, f"{what} must share one dtype, {dtype} and {t.dtype} given")
-            _need(False, f"{what} must be contiguous, shape {tuple(t.shape)} strides {tuple(t.stride())}")
-    _need(dtype in _DT or dtype is None, f"{what} must be fp32 or bf16, is {dtype}")
+        _dev(t)
+        _need(t.is_contiguous(), f"{what} must be contiguous, shape {tuple(t.shape)} strides {tuple(t.stride())}")
+        _need(t.dtype in _DT, f"{what} must be fp32 or bf16, is {t.dtype}")
+    _need(dtype is None or dtypes == {dtype}, f"{what} must be {dtype}, {dtypes} given")
+    _need(len(dtypes) == 1, f"{what} must share one dtype, {dtypes} given")
+    _need(False, f"{what} must be on one device{'' if device is None else f' ({device})'}, {devices} given")
 
 
 def grad_norm(grads: Union[torch.Tensor, Sequence[torch.Tensor]], max_norm: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -945,20 +957,20 @@ def grad_norm(grads: Union[torch.Tensor, Sequence[torch.Tensor]], max_norm: floa
     _need(len(grads) > 0, "grad_norm needs at least one tensor")
     _need(max_norm > 0, f"grad_norm: max_norm must be positive, is {max_norm}")
     _tensor_list(grads, "grad_norm: gradients")
-    n = len(grads)
-    ptrs = (C.c_void_p * n)(*[g.data_ptr() for g in grads])
-    sizes = (C.c_int64 * n)(*[g.numel() for g in grads])
-    dev = grads[0].device
+    n, dev = len(grads), grads[0].get_device()
+    ptrs, sizes = array("q", map(_T.data_ptr, grads)), array("q", map(_T.numel, grads))
+    pa, sa = ptrs.buffer_info()[0], sizes.buffer_info()[0]
     with _on(dev):
         if out is None:
-            out = torch.empty(2, dtype=torch.float32, device=dev)
+            out = torch.empty(2, dtype=torch.float32, device=grads[0].device)
         _numel(out, 2, "grad_norm out", torch.float32)
-        _need(out.device == dev, "grad_norm: out must be on the gradients' device")
-        wsb = lib.cfd_grad_norm_workspace_bytes(sizes, n)
+        _need(out.get_device() == dev, "grad_norm: out must be on the gradients' device")
+        wsb = lib.cfd_grad_norm_workspace_bytes(sa, n)
         if wsb < 0:
             check(-1, "cfd_grad_norm_workspace_bytes")
-        ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
-        check(lib.cfd_grad_norm(ptrs, sizes, n, _DT[grads[0].dtype], float(max_norm), _ptr(ws), _ptr(out), _stream()), "cfd_grad_norm")
+        ws = torch.empty(wsb, dtype=torch.uint8, device=out.device)
+        check(lib.cfd_grad_norm(pa, sa, n, _DT[grads[0].dtype], float(max_norm), ws.data_ptr(), out.data_ptr(), _raw_stream(dev)),
+              "cfd_grad_norm")
     return out
 
 
@@ -967,9 +979,10 @@ ADAMW_BLOCK = 256      # elements that share a scale of an 8-bit state; every te
 
 def adamw_step(table, desc: AdamwDesc, m, v, m_scale, v_scale, t, lr, grad_scale, ws) -> None:
     """cfd_adamw_step on a host table of AdamwTensor records; trainer.AdamW builds and checks the operands"""
-    with _on(m.device):
+    dev = m.get_device()
+    with _on(dev):
         check(_lib.load().cfd_adamw_step(table, len(table), C.byref(desc), _ptr(m), _ptr(v), _ptr(m_scale), _ptr(v_scale), _ptr(t),
-                                         _ptr(lr), _ptr(grad_scale), _ptr(ws), _stream()), "cfd_adamw_step")
+                                         _ptr(lr), _ptr(grad_scale), _ptr(ws), _raw_stream(dev)), "cfd_adamw_step")
 
 
 # ----------------------------------------------------------------------------------------
@@ -995,35 +1008,42 @@ def _mx_empty(rows: int, cols: int, device) -> Mxfp4:
 
 def _mx_check(q: Mxfp4, what: str) -> None:
     _need(isinstance(q, Mxfp4), f"{what} must be an Mxfp4 matrix")
-    _need(0 < q.cols <= 1 << 22, f"{what}: columns must be in 1 .. 4194304")
-    nb, rows = (q.cols + 31) // 32, q.codes.shape[0]
-    for t, width, name in ((q.codes, nb * 16, "codes"), (q.scales, (nb + 15) // 16 * 16, "scales")):
+    codes, scales, cols = q
+    _need(0 < cols <= 1 << 22, f"{what}: columns must be in 1 .. 4194304")
+    nb, rows = (cols + 31) // 32, codes.shape[0]
+    if codes.is_cuda and codes.get_device() == scales.get_device() and codes.dtype == torch.uint8 == scales.dtype and codes.is_contiguous() \
+            and scales.is_contiguous() and codes.shape == (rows, nb * 16) and scales.shape == (rows, (nb + 15) // 16 * 16):
+        return
+    for t, width, name in ((codes, nb * 16, "codes"), (scales, (nb + 15) // 16 * 16, "scales")):
         _dev(t)
         _need(t.dtype == torch.uint8 and tuple(t.shape) == (rows, width) and t.is_contiguous(),
               f"{what} {name} must be dense uint8 {(rows, width)}, is {t.dtype} {tuple(t.shape)}")
-    _need(q.codes.device == q.scales.device, f"{what}: codes and scales on one device")
+    _need(False, f"{what}: codes and scales on one device")
 
 
 def _mx_input(x: torch.Tensor, what: str) -> int:
     """row stride of a 2-D fp32 / bf16 matrix whose rows are dense"""
-    _dev(x)
-    _need(x.dim() == 2 and x.dtype in _DT, f"{what} must be a 2-D fp32 or bf16 matrix, is {x.dtype} {tuple(x.shape)}")
-    rows, cols = x.shape
-    _need(0 < cols <= 1 << 22, f"{what}: columns must be in 1 .. 4194304")
-    _need((cols == 1 or x.stride(1) == 1) and (rows <= 1 or x.stride(0) >= cols),
-          f"{what} must have dense rows that do not overlap, strides {tuple(x.stride())}")
-    return x.stride(0) if rows > 1 else cols
+    if not (x.is_cuda and x.dim() == 2 and x.dtype in _DT):
+        _dev(x)
+        _need(False, f"{what} must be a 2-D fp32 or bf16 matrix, is {x.dtype} {tuple(x.shape)}")
+    (rows, cols), (ld, step) = x.shape, x.stride()
+    if not 0 < cols <= 1 << 22:
+        _need(False, f"{what}: columns must be in 1 .. 4194304")
+    if not ((cols == 1 or step == 1) and (rows <= 1 or ld >= cols)):
+        _need(False, f"{what} must have dense rows that do not overlap, strides {(ld, step)}")
+    return ld if rows > 1 else cols
 
 
 def _mx_quantize(x: torch.Tensor, rows: bool, cols: bool):
     ldx = _mx_input(x, "mxfp4_quantize: x")
     R, K = x.shape
     _need(not cols or 0 < R <= 1 << 22, "mxfp4_quantize: a transposed matrix needs 1 .. 4194304 rows")
-    with _on(x.device):
+    dev = x.get_device()
+    with _on(dev):
         q = _mx_empty(R, K, x.device) if rows else None
         t = _mx_empty(K, R, x.device) if cols else None
-        check(_lib.load().cfd_mxfp4_quantize(_ptr(x), ldx, _DT[x.dtype], R, K, _ptr(q and q.codes), _ptr(q and q.scales),
-                                             _ptr(t and t.codes), _ptr(t and t.scales), _stream()), "cfd_mxfp4_quantize")
+        check(_lib.load().cfd_mxfp4_quantize(x.data_ptr(), ldx, _DT[x.dtype], R, K, q and q.codes.data_ptr(), q and q.scales.data_ptr(),
+                                             t and t.codes.data_ptr(), t and t.scales.data_ptr(), _raw_stream(dev)), "cfd_mxfp4_quantize")
     return q, t
 
 
@@ -1041,14 +1061,14 @@ def mxfp4_quantize_both(x: torch.Tensor) -> Tuple[Mxfp4, Mxfp4]:
 def mxfp4_dequantize(q: Mxfp4, dtype: torch.dtype = torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """the values of a 4-bit matrix (exact in either dtype, scales at the ends of the exponent range aside)"""
     _mx_check(q, "mxfp4_dequantize: q")
-    rows, cols = q.shape
-    with _on(q.codes.device):
+    (rows, cols), dev = q.shape, q.codes.get_device()
+    with _on(dev):
         if out is None:
             out = torch.empty((rows, cols), dtype=dtype, device=q.codes.device)
         ldy = _mx_input(out, "mxfp4_dequantize: out")
-        _need(tuple(out.shape) == (rows, cols) and out.device == q.codes.device, f"mxfp4_dequantize: out must be {(rows, cols)} on q's device")
-        check(_lib.load().cfd_mxfp4_dequantize(_ptr(q.codes), _ptr(q.scales), rows, cols, _ptr(out), ldy, _DT[out.dtype], _stream()),
-              "cfd_mxfp4_dequantize")
+        _need(out.shape == (rows, cols) and out.get_device() == dev, f"mxfp4_dequantize: out must be {(rows, cols)} on q's device")
+        check(_lib.load().cfd_mxfp4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), rows, cols, out.data_ptr(), ldy, _DT[out.dtype],
+                                               _raw_stream(dev)), "cfd_mxfp4_dequantize")
     return out
 
 
@@ -1082,7 +1102,7 @@ def mxfp4_dense(x: Union[Mxfp4, torch.Tensor], w: Mxfp4, bias: Optional[torch.Te
     lib = _lib.load()
     _mx_check(w, "mxfp4_dense: w")
     n, k = w.shape
-    dev = w.codes.device
+    dev = w.codes.get_device()
     four = isinstance(x, Mxfp4)
     if four:
         _mx_check(x, "mxfp4_dense: x")
@@ -1092,22 +1112,23 @@ def mxfp4_dense(x: Union[Mxfp4, torch.Tensor], w: Mxfp4, bias: Optional[torch.Te
         kind = _lib.MX_X_F32 if x.dtype == torch.float32 else _lib.MX_X_BF16
     m = x.shape[0]
     _need(x.shape[1] == k, f"mxfp4_dense: x has {x.shape[1]} columns, w {k}")
-    _need(xt.device == dev and (bias is None or bias.device == dev), "mxfp4_dense: x, w and bias on one device")
+    _need(xt.get_device() == dev and (bias is None or bias.get_device() == dev), "mxfp4_dense: x, w and bias on one device")
     _numel(bias, n, "mxfp4_dense bias", torch.float32)
     odt = out_dtype or (out.dtype if out is not None else torch.float32 if four else x.dtype)
+    _need(odt in _DT, f"mxfp4_dense: out_dtype must be fp32 or bf16, is {odt}")
     with _on(dev):
         if out is None:
-            out = torch.empty((m, n), dtype=odt, device=dev)
-        _need(tuple(out.shape) == (m, n) and out.dtype == odt and odt in _DT and out.device == dev,
+            out = torch.empty((m, n), dtype=odt, device=xt.device)
+        _need(out.shape == (m, n) and out.dtype == odt and out.get_device() == dev,
               f"mxfp4_dense: out must be {odt} {(m, n)} on w's device, is {out.dtype} {tuple(out.shape)}")
         if m == 0 or n == 0:
             return out
-        d = Mxfp4DenseDesc(x_kind=kind, out_dtype=_DT[odt], act=act, leaky_slope=slope, m=m, n=n, k=k, ldx=ldx,
-                           ldy=_mx_input(out, "mxfp4_dense: out"))
+        d = Mxfp4DenseDesc(kind, _DT[odt], act, slope, m, n, k, ldx, _mx_input(out, "mxfp4_dense: out"))
         wsb = lib.cfd_mxfp4_dense_workspace_bytes(m, n, k, kind)
         if wsb < 0:
             check(-1, "cfd_mxfp4_dense_workspace_bytes")
-        ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
-        check(lib.cfd_mxfp4_dense(C.byref(d), _ptr(xt), _ptr(x.scales) if four else None, _ptr(w.codes), _ptr(w.scales), _ptr(bias),
-                                  _ptr(out), _ptr(ws), _stream()), "cfd_mxfp4_dense")
+        ws = torch.empty(wsb, dtype=torch.uint8, device=xt.device) if wsb else None
+        check(lib.cfd_mxfp4_dense(C.byref(d), xt.data_ptr(), x.scales.data_ptr() if four else None, w.codes.data_ptr(),
+                                  w.scales.data_ptr(), None if bias is None else bias.data_ptr(), out.data_ptr(),
+                                  None if ws is None else ws.data_ptr(), _raw_stream(dev)), "cfd_mxfp4_dense")
     return out

@@ -17,6 +17,7 @@ from __future__ import annotations
 import math
 from typing import List, Optional
 
+import numpy as np
 import torch
 
 from . import nets, ops
@@ -91,7 +92,7 @@ class AdamW:
         if self.copies is not None:
             if p0.dtype != torch.float32 or len(self.copies) != n:
                 raise ValueError("AdamW: copies need fp32 parameters, one each")
-            ops._tensor_list(self.copies, "AdamW: copies", torch.bfloat16, self.device)
+            ops._tensor_list(self.copies, "AdamW: copies", torch.bfloat16, self.device.index)
             if any(c.numel() != p.numel() for c, p in zip(self.copies, self.params)):
                 raise ValueError("AdamW: a copy must have its parameter's length")
         if state_bits not in (8, 32):
@@ -120,6 +121,7 @@ class AdamW:
         self._desc = ops.AdamwDesc(p_dtype=ops._DT[p0.dtype], state_bits=state_bits, seed=self.seed & 0xffffffff, eps=epsilon,
                                    beta1=beta_1, beta2=beta_2)
         self._sizes = [p.numel() for p in self.params]
+        self._grad_column = np.frombuffer(self._table, dtype=np.int64)[ops.AdamwTensor.g.offset // 8::ops.C.sizeof(ops.AdamwTensor) // 8]
         for k, p in enumerate(self.params):
             e = self._table[k]
             e.p, e.n, e.state_offset, e.weight_decay = p.data_ptr(), p.numel(), self.offsets[k], self.weight_decay[k]
@@ -127,22 +129,21 @@ class AdamW:
         self._ptrs = self._addresses()
 
     def _addresses(self):
-        return [t.data_ptr() for t in self.params + (self.copies or [])]
+        return list(map(torch.Tensor.data_ptr, self.params + (self.copies or [])))
 
     def step(self, grads, grad_scale=None) -> None:
         """One update from `grads` (one dense fp32 or bf16 tensor per parameter, one dtype).  grad_scale: None, or an fp32
         device tensor of one element that multiplies every gradient (ops.grad_norm(...)[1:]); where it is not finite the
         whole step is skipped, t included."""
         grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
-        if [g.numel() for g in grads] != self._sizes:
+        if list(map(torch.Tensor.numel, grads)) != self._sizes:
             raise ValueError("AdamW.step: one gradient per parameter, of its length")
-        ops._tensor_list(grads, "AdamW.step: gradients", None, self.device)
+        ops._tensor_list(grads, "AdamW.step: gradients", None, self.device.index)
         if self._addresses() != self._ptrs:
             raise RuntimeError("AdamW: a parameter's storage was replaced after the optimizer was built")
         if grad_scale is not None and not (grad_scale.device == self.device and grad_scale.dtype == torch.float32 and grad_scale.numel() == 1):
             raise ValueError("AdamW.step: grad_scale must be one fp32 element on the parameters' device")
-        for e, g in zip(self._table, grads):
-            e.g = g.data_ptr()
+        self._grad_column[:] = list(map(torch.Tensor.data_ptr, grads))
         self._desc.g_dtype = ops._DT[grads[0].dtype]
         on_device = isinstance(self.lr, torch.Tensor)
         self._desc.lr = 0.0 if on_device else float(self.lr)
