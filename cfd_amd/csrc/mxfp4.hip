@@ -73,75 +73,131 @@ __device__ __forceinline__ unsigned quad_umax(unsigned v) {
   return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));  // lane ^ 2
 }
 
-// scale byte of block b, and the zero bytes behind the last block
-__device__ __forceinline__ void put_scale(uint8_t *row, int b, int nb, int pitch, unsigned byte) {
-  row[b] = (uint8_t)byte;
-  if (b == nb - 1)
-    for (int i = nb; i < pitch; ++i) row[i] = 0;
+// one lane stores four consecutive scale bytes from block b on (bytes of blocks that are not there are zero), and the zeros
+// behind them if they are the row's last
+__device__ __forceinline__ void put_scales4(uint8_t *row, int b, int nb, int pitch, unsigned bytes) {
+  *(unsigned *)(row + b) = bytes;
+  if (b + 4 >= nb)
+    for (int i = b + 4; i < pitch; i += 4) *(unsigned *)(row + i) = 0u;
+}
+// the four scale bytes that a row of 16 lanes holds, one per quad
+__device__ __forceinline__ unsigned row16_bytes(unsigned byte) {
+  unsigned v = byte << (((threadIdx.x >> 2) & 3) * 8);
+  v |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x124, 0xf, 0xf, false);
+  return v | (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x128, 0xf, 0xf, false);
+}
+__device__ __forceinline__ unsigned quad_bytes(unsigned byte) {   // the same over the four lanes of a quad
+  unsigned v = byte << ((threadIdx.x & 3) * 8);
+  v |= (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0xB1, 0xf, 0xf, false);
+  return v | (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false);
 }
 
 // rows only: four lanes share a block of 32 (eight columns each): 32-byte / 16-byte loads, 4-byte stores, the block's
-// maximum in two DPP steps.  HBM-bound: s_in + 0.53 bytes an element.
+// maximum in two DPP steps.  HBM-bound: s_in + 0.53 bytes an element.  A row is walked in multiples of 128 columns, so that 16
+// lanes hold four whole scale bytes.
 template <typename T> __global__ __launch_bounds__(256) void mx_quant_rows_kernel(const T *x, int64_t ldx, int64_t rows, int K,
                                                                                    int nb, int pitch, uint8_t *codes,
                                                                                    uint8_t *scales) {
-  const int64_t G = (int64_t)nb * 4, total = rows * G;
+  const int64_t G = (int64_t)((nb + 3) / 4) * 16, total = rows * G;
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t >= total) return;                 // (whole quads: G is a multiple of 4)
+  if (t >= total) return;                 // (whole rows of 16 lanes: G is a multiple of 16)
   const int64_t row = t / G;
   const int grp = (int)(t - row * G);
   float v[8];
   load8(x + row * ldx + (int64_t)grp * 8, K - grp * 8, v);
   const unsigned byte = mx_scale_byte(quad_umax(amax8(v)));
-  *(unsigned *)(codes + row * nb * 16 + (int64_t)grp * 4) = mx_code8(v, byte);
-  if ((grp & 3) == 0) put_scale(scales + row * pitch, grp >> 2, nb, pitch, byte);
+  if ((grp >> 2) < nb) *(unsigned *)(codes + row * nb * 16 + (int64_t)grp * 4) = mx_code8(v, byte);
+  const unsigned bytes = row16_bytes(byte);
+  if ((grp & 15) == 0) put_scales4(scales + row * pitch, grp >> 2, nb, pitch, bytes);
 }
 
-// both orientations from one read: a 128 x 64 tile; rows are coded on the way in, columns from LDS.  The tile's columns
-// are swizzled by 16 per 32 rows so that the four row blocks a quad of lanes reads fall into different banks.
-constexpr int QT_R = 128, QT_C = 64;
+// both orientations from one read: a 128 x 128 tile; rows are coded on the way in, columns from LDS, two adjacent columns and 32
+// rows a thread.  LDS words are swizzled by 16 per 32 rows: the four row blocks that a quad of lanes reads lie in different banks.
+// Codes leave as 64 contiguous bytes a row in both orientations, scales as 32-bit words.
+constexpr int QT = 128;
+template <typename T> struct Raw8;      // eight values as they lie in memory
+template <> struct Raw8<bf16> { bf16x8a2 a; };
+template <> struct Raw8<float> { f32x4a4 a, b; };
 template <typename T> __global__ __launch_bounds__(256) void mx_quant_both_kernel(const T *x, int64_t ldx, int R, int K,
                                                                                    int nb, int pitch, uint8_t *codes,
                                                                                    uint8_t *scales, int nbt, int pitch_t,
                                                                                    uint8_t *codes_t, uint8_t *scales_t) {
-  __shared__ float tile[QT_R * QT_C];
-  const int r0 = blockIdx.y * QT_R, c0 = blockIdx.x * QT_C;
-  const int tid = threadIdx.x;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int r = i * 32 + (tid >> 3), c = (tid & 7) * 8;
-    float v[8];
-    load8(x + (int64_t)(r0 + r) * ldx + c0 + c, r0 + r < R ? K - c0 - c : 0, v);
-    float *dst = tile + r * QT_C + (c ^ ((r >> 5) * 16));
-    *(f32x4 *)dst = (f32x4){v[0], v[1], v[2], v[3]};
-    *(f32x4 *)(dst + 4) = (f32x4){v[4], v[5], v[6], v[7]};
+  constexpr int W = QT * (int)sizeof(T) / 4;       // words of a tile row
+  __shared__ __attribute__((aligned(16))) unsigned tile[QT * W];
+  const int r0 = blockIdx.y * QT, c0 = blockIdx.x * QT;
+  const int tid = threadIdx.x, c = (tid & 15) * 8;
+  auto put = [&](int i, const float (&v)[8]) {     // eight values of a row into LDS, coded along the row
+    const int r = i * 16 + (tid >> 4);
+    unsigned *dst = tile + r * W + ((c * (int)sizeof(T) / 4) ^ ((r >> 5) * 16));
+    if constexpr (sizeof(T) == 2) {
+      *(bf16x8 *)dst = (bf16x8){(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3], (bf16)v[4], (bf16)v[5], (bf16)v[6], (bf16)v[7]};
+    } else {
+      *(f32x4 *)dst = (f32x4){v[0], v[1], v[2], v[3]};
+      *(f32x4 *)(dst + 4) = (f32x4){v[4], v[5], v[6], v[7]};
+    }
     if (codes) {
-      const unsigned byte = mx_scale_byte(quad_umax(amax8(v)));
+      const unsigned byte = mx_scale_byte(quad_umax(amax8(v))), bytes = row16_bytes(byte);
       const int b = (c0 + c) >> 5;
-      if (r0 + r < R && b < nb) {
-        *(unsigned *)(codes + (int64_t)(r0 + r) * nb * 16 + (c0 + c) / 2) = mx_code8(v, byte);
-        if ((tid & 3) == 0) put_scale(scales + (int64_t)(r0 + r) * pitch, b, nb, pitch, byte);
+      if (r0 + r < R) {
+        if (b < nb) *(unsigned *)(codes + (int64_t)(r0 + r) * nb * 16 + (c0 + c) / 2) = mx_code8(v, byte);
+        if ((tid & 15) == 0) put_scales4(scales + (int64_t)(r0 + r) * pitch, b, nb, pitch, bytes);
       }
+    }
+  };
+  const T *src0 = x + (int64_t)(r0 + (tid >> 4)) * ldx + c0 + c;
+  if (r0 + QT <= R && c0 + QT <= K) {              // a whole tile: eight loads in flight
+    Raw8<T> raw[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) raw[i] = *(const Raw8<T> *)(src0 + i * 16 * ldx);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        if constexpr (sizeof(T) == 2) v[e] = (float)raw[i].a[e];
+        else v[e] = e < 4 ? raw[i].a[e & 3] : raw[i].b[e & 3];
+      }
+      put(i, v);
+    }
+  } else {
+    for (int i = 0; i < 8; ++i) {
+      float v[8];
+      load8(src0 + i * 16 * ldx, r0 + i * 16 + (tid >> 4) < R ? K - c0 - c : 0, v);
+      put(i, v);
     }
   }
   __syncthreads();
-  const int c = tid >> 2, rb = tid & 3;      // one column's 32 rows
-  const int bt = (r0 >> 5) + rb;
-  if (c0 + c >= K || bt >= nbt) return;
-  float v[4][8];
-  unsigned am = 0;
+  const int rb = tid & 3, cc = (tid >> 2) * 2, bt = (r0 >> 5) + rb;    // this thread's row block and two columns
+  const unsigned *src = tile + rb * 32 * W + ((cc * (int)sizeof(T) / 4) ^ (rb * 16));
+  float v[2][4][8];
+  unsigned am[2] = {0, 0};
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[g][i] = tile[(rb * 32 + g * 8 + i) * QT_C + (c ^ (rb * 16))];
-    am = max(am, amax8(v[g]));
+    for (int i = 0; i < 8; ++i) {
+      const unsigned *w = src + (g * 8 + i) * W;
+      if constexpr (sizeof(T) == 2) {
+        const bf16x2 p = *(const bf16x2 *)w;
+        v[0][g][i] = (float)p[0]; v[1][g][i] = (float)p[1];
+      } else {
+        const f32x2 p = *(const f32x2 *)w;
+        v[0][g][i] = p[0]; v[1][g][i] = p[1];
+      }
+    }
+    am[0] = max(am[0], amax8(v[0][g]));
+    am[1] = max(am[1], amax8(v[1][g]));
   }
-  const unsigned byte = mx_scale_byte(am);
-  i32x4 o;
 #pragma unroll
-  for (int g = 0; g < 4; ++g) o[g] = (int)mx_code8(v[g], byte);
-  *(i32x4 *)(codes_t + (int64_t)(c0 + c) * nbt * 16 + bt * 16) = o;
-  put_scale(scales_t + (int64_t)(c0 + c) * pitch_t, bt, nbt, pitch_t, byte);
+  for (int k = 0; k < 2; ++k) {
+    const unsigned byte = mx_scale_byte(am[k]), bytes = quad_bytes(byte);
+    const int64_t col = c0 + cc + k;
+    if (col >= K) continue;
+    i32x4 o;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) o[g] = (int)mx_code8(v[k][g], byte);
+    if (bt < nbt) *(i32x4 *)(codes_t + col * nbt * 16 + bt * 16) = o;
+    if (rb == 0) put_scales4(scales_t + col * pitch_t, bt, nbt, pitch_t, bytes);
+  }
 }
 
 // codes -> values: a lane reads eight codes and writes 16 (bf16) or 32 (fp32) bytes
@@ -766,7 +822,7 @@ extern "C" int cfd_mxfp4_quantize(const void *x, int64_t ldx, int dtype, int64_t
   hipStream_t st = (hipStream_t)stream;
   const int nb = (int)mx_blocks(cols), pitch = (int)mx_scale_pitch(cols);
   if (!codes_t) {
-    const int64_t blocks = (rows * nb * 4 + 255) / 256;
+    const int64_t blocks = (rows * ((nb + 3) / 4 * 16) + 255) / 256;
     CFD_REQUIRE(blocks <= 0x7fffffff, "too many elements");
     if (dtype == CFD_BF16)
       hipLaunchKernelGGL(mx_quant_rows_kernel<bf16>, dim3((unsigned)blocks), dim3(256), 0, st, (const bf16 *)x, ldx, rows,
@@ -777,7 +833,7 @@ extern "C" int cfd_mxfp4_quantize(const void *x, int64_t ldx, int dtype, int64_t
   } else {
     if (int rc = mx_check(cols, 0, rows)) return rc;   // the rows are the other orientation's columns
     const int nbt = (int)mx_blocks(rows), pitch_t = (int)mx_scale_pitch(rows);
-    const dim3 grid((unsigned)((cols + QT_C - 1) / QT_C), (unsigned)((rows + QT_R - 1) / QT_R));
+    const dim3 grid((unsigned)((cols + QT - 1) / QT), (unsigned)((rows + QT - 1) / QT));
     if (dtype == CFD_BF16)
       hipLaunchKernelGGL(mx_quant_both_kernel<bf16>, grid, dim3(256), 0, st, (const bf16 *)x, ldx, (int)rows, (int)cols, nb,
                          pitch, codes, scales, nbt, pitch_t, codes_t, scales_t);

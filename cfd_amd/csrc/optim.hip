@@ -179,7 +179,9 @@ __device__ __forceinline__ void adamw_elem(float &p, float g, float &m, float &v
   m = m + (g - m) * c1;
   v = v + (g * g - v) * c2;
   p = p - p * lrwd;
-  p = p - (h.alpha * m) / (sqrtf(v) + eps);
+  // (hardware square root and reciprocal, one ulp each, subnormal v as zero: eps >= 1e-12 hides what that loses; the IEEE
+  // sequences are a third of the 8-bit kernel's instructions)
+  p = p - (h.alpha * m) * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v) + eps);
 }
 
 // fp32 state: one 16-byte vector per stream and thread (32 B in, 12-14 B out per element of work)
@@ -193,17 +195,19 @@ template <typename TP, typename TG> __global__ __launch_bounds__(256) void adamw
   float *m = (float *)a.m + a.off[ti], *v = (float *)a.v + a.off[ti];
   bf16 *copy = a.copy[ti];
   const float lrwd = h.lr * a.wd[ti];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int64_t e = e0 + j * 1024 + threadIdx.x * 4;
-    if (e >= n) break;
-    const int left = (int)min(n - e, (int64_t)4);
+  auto four = [&](int64_t e, int left) {
     float pv[4], gv[4], mv[4], vv[4];
     load4(p + e, left, pv); load4(g + e, left, gv); load4(m + e, left, mv); load4(v + e, left, vv);
 #pragma unroll
     for (int k = 0; k < 4; ++k) adamw_elem(pv[k], gv[k], mv[k], vv[k], h, a.c1, a.c2, a.eps, lrwd);
     store4(p + e, left, pv); store4(m + e, left, mv); store4(v + e, left, vv);
     if (copy) store4(copy + e, left, pv);
+  };
+  if (e0 + OPT_CHUNK <= n) {   // whole: no lane has a tail
+#pragma unroll
+    for (int j = 0; j < 4; ++j) four(e0 + j * 1024 + threadIdx.x * 4, 4);
+  } else {
+    for (int64_t e = e0 + threadIdx.x * 4; e < n; e += 1024) four(e, (int)min(n - e, (int64_t)4));
   }
 }
 
@@ -221,15 +225,9 @@ template <int SHIFT, int DROP> __device__ __forceinline__ unsigned round_code(fl
   return (z + (rnd16 << (DROP - 16))) >> DROP;
 }
 
-template <typename TP, typename TG> __global__ __launch_bounds__(256) void adamw8_kernel(AdamwArgs a) {
-  const int ti = find_tensor(a.first, a.nt, blockIdx.x);
-  const AdamwHyper h = *a.h;
-  if (h.skip) return;
-  const int lane = threadIdx.x & 63, q = lane >> 4, l = lane & 15;
-  const int64_t n = a.n[ti];
-  const int64_t e0 = (int64_t)(blockIdx.x - a.first[ti]) * OPT_CHUNK + (threadIdx.x >> 6) * 1024 + q * OPT_BLOCK;
-  // (a row of 16 lanes has one block: it leaves together, and the DPP steps below stay inside the row)
-  if (e0 >= n) return;
+template <typename TP, typename TG, bool WHOLE> __device__ __forceinline__ void adamw8_block(const AdamwArgs &a, const AdamwHyper &h,
+                                                                                               int ti, int64_t e0, int64_t n) {
+  const int l = threadIdx.x & 15;
   TP *p = (TP *)a.p[ti];
   const TG *g = (const TG *)a.g[ti];
   const int64_t s0 = a.off[ti] + e0;   // position in the state (a multiple of 256)
@@ -245,7 +243,7 @@ template <typename TP, typename TG> __global__ __launch_bounds__(256) void adamw
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const int64_t e = e0 + j * 64 + l * 4;
-    left[j] = (int)max((int64_t)0, min(n - e, (int64_t)4));
+    left[j] = WHOLE ? 4 : (int)max((int64_t)0, min(n - e, (int64_t)4));
     mc[j] = mq[j * 16 + l];            // (the state is padded to whole blocks)
     vc[j] = vq[j * 16 + l];
     load4(p + e, left[j], pv[j]);
@@ -279,7 +277,7 @@ template <typename TP, typename TG> __global__ __launch_bounds__(256) void adamw
       const unsigned r = hash32((unsigned)(s0 + j * 64 + l * 4 + k) ^ h.key);
       const unsigned qm = round_code<120, 20>(mv[j][k], mf - 127, r & 0xffffu) | ((__float_as_uint(mv[j][k]) >> 24) & 0x80u);
       unsigned qv = round_code<112, 21>(vv[j][k], vf - 127, r >> 16);
-      if (qv == 0 && vv[j][k] > 0.f) qv = 1;
+      qv = max(qv, vv[j][k] > 0.f ? 1u : 0u);
       mo |= qm << (8 * k);
       vo |= qv << (8 * k);
     }
@@ -290,6 +288,16 @@ template <typename TP, typename TG> __global__ __launch_bounds__(256) void adamw
     *msp = mbad ? NAN : __uint_as_float((unsigned)mf << 23);
     *vsp = vbad ? NAN : __uint_as_float((unsigned)vf << 23);
   }
+}
+
+template <typename TP, typename TG> __global__ __launch_bounds__(256) void adamw8_kernel(AdamwArgs a) {
+  const int ti = find_tensor(a.first, a.nt, blockIdx.x);
+  const AdamwHyper h = *a.h;
+  if (h.skip) return;
+  const int64_t n = a.n[ti], w0 = (int64_t)(blockIdx.x - a.first[ti]) * OPT_CHUNK + (threadIdx.x >> 6) * 1024;
+  const int64_t e0 = w0 + ((threadIdx.x & 63) >> 4) * OPT_BLOCK;
+  if (w0 + 1024 <= n) adamw8_block<TP, TG, true>(a, h, ti, e0, n);
+  else if (e0 < n) adamw8_block<TP, TG, false>(a, h, ti, e0, n);   // (a row of 16 lanes stays or leaves together)
 }
 
 // elements per workgroup of the norm: whole rounds of 4 096, at most ~2 048 workgroups (the last kernel adds their sums)
@@ -352,7 +360,7 @@ extern "C" int cfd_adamw_step(const cfd_adamw_tensor *t, int count, const cfd_ad
   CFD_REQUIRE(t && count > 0 && d && m && v && step && ws, "bad arguments");
   CFD_REQUIRE(d->state_bits == 32 || (d->state_bits == 8 && m_scale && v_scale), "state_bits must be 32, or 8 with scales");
   CFD_REQUIRE((d->p_dtype == CFD_F32 || d->p_dtype == CFD_BF16) && (d->g_dtype == CFD_F32 || d->g_dtype == CFD_BF16), "bad dtype");
-  CFD_REQUIRE(d->beta1 >= 0. && d->beta1 < 1. && d->beta2 >= 0. && d->beta2 < 1. && d->eps >= 0.f, "beta must be in [0, 1), eps >= 0");
+  CFD_REQUIRE(d->beta1 >= 0. && d->beta1 < 1. && d->beta2 >= 0. && d->beta2 < 1. && d->eps >= 1e-12f, "beta must be in [0, 1), eps at least 1e-12");
   CFD_REQUIRE((((uintptr_t)m | (uintptr_t)v) & 15) == 0, "state must be 16-byte aligned");
   int64_t blocks = 0;
   for (int i = 0; i < count; ++i) {

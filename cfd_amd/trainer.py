@@ -97,8 +97,8 @@ class AdamW:
                 raise ValueError("AdamW: a copy must have its parameter's length")
         if state_bits not in (8, 32):
             raise ValueError("AdamW: state_bits must be 8 or 32")
-        if not (0.0 <= beta_1 < 1.0 and 0.0 <= beta_2 < 1.0 and epsilon >= 0.0):
-            raise ValueError("AdamW: beta must be in [0, 1) and epsilon >= 0")
+        if not (0.0 <= beta_1 < 1.0 and 0.0 <= beta_2 < 1.0 and epsilon >= 1e-12):
+            raise ValueError("AdamW: beta must be in [0, 1) and epsilon at least 1e-12")
         if isinstance(lr, torch.Tensor) and not (lr.device == self.device and lr.dtype == torch.float32 and lr.numel() == 1):
             raise ValueError("AdamW: a learning-rate tensor must be one fp32 element on the parameters' device")
         spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in self.params + (self.copies or []) if t.numel())

@@ -349,8 +349,8 @@ typedef struct {
   int p_dtype, g_dtype; /* cfd_dtype */
   int state_bits;       /* 32 or 8 */
   unsigned seed;        /* of the 8-bit state's rounding */
-  float lr, eps;
-  double beta1, beta2;
+  float lr, eps;        /* eps >= 1e-12 */
+  double beta1, beta2;  /* in [0, 1) */
 } cfd_adamw_desc;
 int cfd_adamw_step(const cfd_adamw_tensor *tensors, int count, const cfd_adamw_desc *desc, void *m, void *v, float *m_scale,
                    float *v_scale, int *step, const float *lr_device, const float *grad_scale, void *ws, void *stream);
