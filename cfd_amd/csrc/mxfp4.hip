@@ -73,6 +73,58 @@ __device__ __forceinline__ unsigned quad_umax(unsigned v) {
   return max(v, (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, 0x4E, 0xf, 0xf, false));  // lane ^ 2
 }
 
+// the same for eight bf16 as they lie in memory (four words): two magnitudes a comparison, and no way through fp32
+__device__ __forceinline__ unsigned pk_max_u16(unsigned a, unsigned b) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b)));
+}
+__device__ __forceinline__ unsigned amax8(const i32x4 &w) {
+  const unsigned m = pk_max_u16(pk_max_u16((unsigned)w[0] & 0x7fff7fffu, (unsigned)w[1] & 0x7fff7fffu),
+                                pk_max_u16((unsigned)w[2] & 0x7fff7fffu, (unsigned)w[3] & 0x7fff7fffu));
+  return max(m & 0xffff0000u, m << 16);
+}
+__device__ __forceinline__ bf16x2 two_bf16(int w) { return __builtin_bit_cast(bf16x2, w); }   // (of a copy: not of a vector's element)
+__device__ __forceinline__ unsigned mx_code8(const i32x4 &w, unsigned byte) {
+  const float s = mx_scale_f32(byte);
+  unsigned c = 0;
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, two_bf16(w[0]), s, 0);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, two_bf16(w[1]), s, 1);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, two_bf16(w[2]), s, 2);
+  c = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(c, two_bf16(w[3]), s, 3);
+  return byte == 255u ? 0u : c;
+}
+// eight values as the quantisation works on them: fp32 as numbers, bf16 as words
+template <typename T> struct Eight;
+template <> struct Eight<float> {
+  float v[8];
+  __device__ __forceinline__ void load(const float *p) {
+    const f32x4a4 a = *(const f32x4a4 *)p, b = *(const f32x4a4 *)(p + 4);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { v[i] = a[i]; v[4 + i] = b[i]; }
+  }
+  __device__ __forceinline__ void load(const float *p, int left) { load8(p, left, v); }
+  __device__ __forceinline__ void to_lds(unsigned *d) const {
+    *(f32x4 *)d = (f32x4){v[0], v[1], v[2], v[3]};
+    *(f32x4 *)(d + 4) = (f32x4){v[4], v[5], v[6], v[7]};
+  }
+  __device__ __forceinline__ const float (&get() const)[8] { return v; }
+};
+typedef int i32x4a2 __attribute__((ext_vector_type(4), aligned(2)));
+template <> struct Eight<bf16> {
+  i32x4 w;
+  __device__ __forceinline__ void load(const bf16 *p) { w = *(const i32x4a2 *)p; }
+  __device__ __forceinline__ void load(const bf16 *p, int left) {
+    if (left >= 8) { load(p); return; }
+    unsigned short h[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) h[i] = i < left ? ((const unsigned short *)p)[i] : (unsigned short)0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (int)(h[2 * i] | ((unsigned)h[2 * i + 1] << 16));
+  }
+  __device__ __forceinline__ void to_lds(unsigned *d) const { *(i32x4 *)d = w; }
+  __device__ __forceinline__ const i32x4 &get() const { return w; }
+};
+
 // one lane stores four consecutive scale bytes from block b on (bytes of blocks that are not there are zero), and the zeros
 // behind them if they are the row's last
 __device__ __forceinline__ void put_scales4(uint8_t *row, int b, int nb, int pitch, unsigned bytes) {
@@ -103,10 +155,10 @@ template <typename T> __global__ __launch_bounds__(256) void mx_quant_rows_kerne
   if (t >= total) return;                 // (whole rows of 16 lanes: G is a multiple of 16)
   const int64_t row = t / G;
   const int grp = (int)(t - row * G);
-  float v[8];
-  load8(x + row * ldx + (int64_t)grp * 8, K - grp * 8, v);
-  const unsigned byte = mx_scale_byte(quad_umax(amax8(v)));
-  if ((grp >> 2) < nb) *(unsigned *)(codes + row * nb * 16 + (int64_t)grp * 4) = mx_code8(v, byte);
+  Eight<T> v;
+  v.load(x + row * ldx + (int64_t)grp * 8, K - grp * 8);
+  const unsigned byte = mx_scale_byte(quad_umax(amax8(v.get())));
+  if ((grp >> 2) < nb) *(unsigned *)(codes + row * nb * 16 + (int64_t)grp * 4) = mx_code8(v.get(), byte);
   const unsigned bytes = row16_bytes(byte);
   if ((grp & 15) == 0) put_scales4(scales + row * pitch, grp >> 2, nb, pitch, bytes);
 }
@@ -115,9 +167,6 @@ template <typename T> __global__ __launch_bounds__(256) void mx_quant_rows_kerne
 // rows a thread.  LDS words are swizzled by 16 per 32 rows: the four row blocks that a quad of lanes reads lie in different banks.
 // Codes leave as 64 contiguous bytes a row in both orientations, scales as 32-bit words.
 constexpr int QT = 128;
-template <typename T> struct Raw8;      // eight values as they lie in memory
-template <> struct Raw8<bf16> { bf16x8a2 a; };
-template <> struct Raw8<float> { f32x4a4 a, b; };
 template <typename T> __global__ __launch_bounds__(256) void mx_quant_both_kernel(const T *x, int64_t ldx, int R, int K,
                                                                                    int nb, int pitch, uint8_t *codes,
                                                                                    uint8_t *scales, int nbt, int pitch_t,
@@ -126,66 +175,53 @@ template <typename T> __global__ __launch_bounds__(256) void mx_quant_both_kerne
   __shared__ __attribute__((aligned(16))) unsigned tile[QT * W];
   const int r0 = blockIdx.y * QT, c0 = blockIdx.x * QT;
   const int tid = threadIdx.x, c = (tid & 15) * 8;
-  auto put = [&](int i, const float (&v)[8]) {     // eight values of a row into LDS, coded along the row
+  auto put = [&](int i, const Eight<T> &v) {       // eight values of a row into LDS, coded along the row
     const int r = i * 16 + (tid >> 4);
-    unsigned *dst = tile + r * W + ((c * (int)sizeof(T) / 4) ^ ((r >> 5) * 16));
-    if constexpr (sizeof(T) == 2) {
-      *(bf16x8 *)dst = (bf16x8){(bf16)v[0], (bf16)v[1], (bf16)v[2], (bf16)v[3], (bf16)v[4], (bf16)v[5], (bf16)v[6], (bf16)v[7]};
-    } else {
-      *(f32x4 *)dst = (f32x4){v[0], v[1], v[2], v[3]};
-      *(f32x4 *)(dst + 4) = (f32x4){v[4], v[5], v[6], v[7]};
-    }
+    v.to_lds(tile + r * W + ((c * (int)sizeof(T) / 4) ^ ((r >> 5) * 16)));
     if (codes) {
-      const unsigned byte = mx_scale_byte(quad_umax(amax8(v))), bytes = row16_bytes(byte);
+      const unsigned byte = mx_scale_byte(quad_umax(amax8(v.get()))), bytes = row16_bytes(byte);
       const int b = (c0 + c) >> 5;
       if (r0 + r < R) {
-        if (b < nb) *(unsigned *)(codes + (int64_t)(r0 + r) * nb * 16 + (c0 + c) / 2) = mx_code8(v, byte);
+        if (b < nb) *(unsigned *)(codes + (int64_t)(r0 + r) * nb * 16 + (c0 + c) / 2) = mx_code8(v.get(), byte);
         if ((tid & 15) == 0) put_scales4(scales + (int64_t)(r0 + r) * pitch, b, nb, pitch, bytes);
       }
     }
   };
   const T *src0 = x + (int64_t)(r0 + (tid >> 4)) * ldx + c0 + c;
   if (r0 + QT <= R && c0 + QT <= K) {              // a whole tile: eight loads in flight
-    Raw8<T> raw[8];
+    Eight<T> v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) raw[i] = *(const Raw8<T> *)(src0 + i * 16 * ldx);
+    for (int i = 0; i < 8; ++i) v[i].load(src0 + i * 16 * ldx);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if constexpr (sizeof(T) == 2) v[e] = (float)raw[i].a[e];
-        else v[e] = e < 4 ? raw[i].a[e & 3] : raw[i].b[e & 3];
-      }
-      put(i, v);
-    }
+    for (int i = 0; i < 8; ++i) put(i, v[i]);
   } else {
     for (int i = 0; i < 8; ++i) {
-      float v[8];
-      load8(src0 + i * 16 * ldx, r0 + i * 16 + (tid >> 4) < R ? K - c0 - c : 0, v);
+      Eight<T> v;
+      v.load(src0 + i * 16 * ldx, r0 + i * 16 + (tid >> 4) < R ? K - c0 - c : 0);
       put(i, v);
     }
   }
   __syncthreads();
   const int rb = tid & 3, cc = (tid >> 2) * 2, bt = (r0 >> 5) + rb;    // this thread's row block and two columns
   const unsigned *src = tile + rb * 32 * W + ((cc * (int)sizeof(T) / 4) ^ (rb * 16));
-  float v[2][4][8];
+  Eight<T> v[2][4];
   unsigned am[2] = {0, 0};
 #pragma unroll
   for (int g = 0; g < 4; ++g) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const unsigned *w = src + (g * 8 + i) * W;
-      if constexpr (sizeof(T) == 2) {
-        const bf16x2 p = *(const bf16x2 *)w;
-        v[0][g][i] = (float)p[0]; v[1][g][i] = (float)p[1];
+    for (int i = 0; i < 8; i += 2) {
+      const unsigned *w0 = src + (g * 8 + i) * W, *w1 = w0 + W;
+      if constexpr (sizeof(T) == 2) {              // two rows of two columns -> two columns of two rows
+        v[0][g].w[i / 2] = (int)__builtin_amdgcn_perm(*w1, *w0, 0x05040100u);
+        v[1][g].w[i / 2] = (int)__builtin_amdgcn_perm(*w1, *w0, 0x07060302u);
       } else {
-        const f32x2 p = *(const f32x2 *)w;
-        v[0][g][i] = p[0]; v[1][g][i] = p[1];
+        const f32x2 p0 = *(const f32x2 *)w0, p1 = *(const f32x2 *)w1;
+        v[0][g].v[i] = p0[0]; v[1][g].v[i] = p0[1];
+        v[0][g].v[i + 1] = p1[0]; v[1][g].v[i + 1] = p1[1];
       }
     }
-    am[0] = max(am[0], amax8(v[0][g]));
-    am[1] = max(am[1], amax8(v[1][g]));
+    am[0] = max(am[0], amax8(v[0][g].get()));
+    am[1] = max(am[1], amax8(v[1][g].get()));
   }
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
@@ -194,7 +230,7 @@ template <typename T> __global__ __launch_bounds__(256) void mx_quant_both_kerne
     if (col >= K) continue;
     i32x4 o;
 #pragma unroll
-    for (int g = 0; g < 4; ++g) o[g] = (int)mx_code8(v[k][g], byte);
+    for (int g = 0; g < 4; ++g) o[g] = (int)mx_code8(v[k][g].get(), byte);
     if (bt < nbt) *(i32x4 *)(codes_t + col * nbt * 16 + bt * 16) = o;
     if (rb == 0) put_scales4(scales_t + col * pitch_t, bt, nbt, pitch_t, bytes);
   }
@@ -396,7 +432,8 @@ __global__ __launch_bounds__(256, 2) void mx_dense_kernel(MxDense p) {
 // registers).  LDS bandwidth decides the wave tile: a 256-column step of eight 128 x 64 waves reads 192 KiB and stages 64 KiB, as
 // long as its MFMAs take at 128 B/clk; four 128 x 128 waves read 128 KiB.
 //   * a K tile is 256 columns = 128 bytes a row (whole cache lines: 64-byte rows filled LDS a quarter slower), two stages for each
-//     operand, filled by LDS-DMA that stays in flight across barriers; 16-byte chunks are XOR-ed with the row's low three bits;
+//     operand, filled by LDS-DMA that stays in flight across barriers; 16-byte chunks are XOR-ed with bits 1-3 of
+//     the row: the 16 lanes that ds_read_b128 serves together (0-3, 12-15, 20-23, 24-27 and so on) then cover all banks once;
 //   * 32x32x64 scaled MFMA, lane = row l & 31, K half h = l >> 5; step s of a K tile takes block 4h + s, so one 32-bit word holds a
 //     lane's four scales of the K tile and the step picks the byte;
 //   * scales: 16 bytes a row cover two K tiles (8 KiB, two stages, two LDS-DMA loads per wave every second K tile);
@@ -460,7 +497,10 @@ template <typename TO> __global__ __launch_bounds__(256, 1) void mx_dense256_ker
   // ---- staging: a wave fills 64 rows of each operand, eight loads of 8 rows; lane -> row lane / 8, source chunk swizzled
   unsigned voff[8];
 #pragma unroll
-  for (int q = 0; q < 8; ++q) voff[q] = (unsigned)((wave * 64 + q * 8 + (lane >> 3)) * cp + (((lane & 7) ^ (lane >> 3)) << 4));
+  for (int q = 0; q < 8; ++q) {
+    const int row = wave * 64 + q * 8 + (lane >> 3);
+    voff[q] = (unsigned)(row * cp + (((lane & 7) ^ ((row >> 1) & 7)) << 4));
+  }
   struct Stream {      // one operand: base of the next K tile, bytes from there to the operand's end, K tiles not issued yet
     const uint8_t *at;
     int left, todo;
@@ -489,7 +529,7 @@ template <typename TO> __global__ __launch_bounds__(256, 1) void mx_dense256_ker
 
   // ---- fragments: weight rows (i >> 1) * 128 + wr * 64 + (i & 1) * 32 + fr, activation rows wc * 128 + j * 32 + fr
   const int fr = lane & 31, fh = lane >> 5;
-  const int laneoff = fr * 128 + (((fh * 4) ^ (fr & 7)) << 4);
+  const int laneoff = fr * 128 + (((fh * 4) ^ ((fr >> 1) & 7)) << 4);
   const char *wrd[4], *xrd[4];
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
