@@ -366,9 +366,10 @@ __device__ __forceinline__ void mx_small_tile(const MxDense &p, int &mt, int &nt
 }
 
 // Both operands in 4 bits, small or long products (bound by reading them): a workgroup owns 64 (m) x 64 (n), its four waves take
-// K groups of 256 columns in turn and join in LDS.  Fragments go from global memory straight into the scaled MFMA
-// (16x16x128: lane = row l & 15, block l >> 4, its scale byte its own); lane group g takes blocks 2g and 2g + 1 of a K
-// group, so one 16-bit load holds both of its scales and the step picks the byte.  A wave loads two K groups at a time.
+// K groups of 512 columns in turn and join in LDS.  Fragments go from global memory straight into the scaled MFMA
+// (16x16x128: lane = row l & 15, block l >> 4, its scale byte its own); step s of a group takes block 4s + (l >> 4), so a load
+// instruction covers 64 contiguous bytes of 16 rows.  The 16 scale bytes of a row's group come with one load (a load for each
+// step cost as much as the codes: 30 -> 24 us at 128 x 256 x 262144 without them); a lane shifts its byte down.
 // Codes behind the last column (the next row's) need no mask: their scale bytes are zero on both operands, 2^-254 is zero in fp32.
 __global__ __launch_bounds__(256, 2) void mx_dense_kernel(MxDense p) {
   __shared__ f32x4 part[4][16][64];
@@ -381,38 +382,34 @@ __global__ __launch_bounds__(256, 2) void mx_dense_kernel(MxDense p) {
   const __amdgpu_buffer_rsrc_t xr = mx_rsrc(p.xc, m0, mr, cp), wr = mx_rsrc(p.wc, n0, nr, cp);
   const __amdgpu_buffer_rsrc_t xsr = mx_rsrc(p.xs, m0, mr, p.pitch), wsr = mx_rsrc(p.ws, n0, nr, p.pitch);
   f32x4 acc[4][4] = {};
-  struct Group { i32x4 a[4][2], b[4][2]; int as[4], bs[4]; };
-  auto load = [&](Group &g, int kt) {
-    const int b0 = kt * 8 + fq * 2;
+  const int k1 = min((sk + 1) * p.kt_per, p.pitch / 16);
+  for (int kt = sk * p.kt_per + wave; kt < k1; kt += 4) {
+    i32x4 a[4][4], b[4][4], as[4], bs[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      // rows past the operand lie past its size and read as zero; kt < 0: nothing left to load
-      const unsigned row = (unsigned)(i * 16 + fr), co = kt < 0 ? MX_OOB : row * cp + b0 * 16, so = kt < 0 ? MX_OOB : row * p.pitch + b0;
+      const unsigned row = (unsigned)(i * 16 + fr);    // (rows past the operand lie past its size and read as zero)
+      as[i] = ld16(wsr, row * p.pitch + kt * 16);
+      bs[i] = ld16(xsr, row * p.pitch + kt * 16);
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        g.a[i][s] = ld16(wr, co + s * 16);
-        g.b[i][s] = ld16(xr, co + s * 16);
+      for (int s = 0; s < 4; ++s) {
+        a[i][s] = ld16(wr, row * cp + kt * 256 + fq * 16 + s * 64);
+        b[i][s] = ld16(xr, row * cp + kt * 256 + fq * 16 + s * 64);
       }
-      g.as[i] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(wsr, (int)so, 0, 0);
-      g.bs[i] = (unsigned short)__builtin_amdgcn_raw_buffer_load_b16(xsr, (int)so, 0, 0);
     }
-  };
-  auto multiply = [&](const Group &g) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int s = 0; s < 4; ++s) {
+      int sa[4], sb[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(g.a[i][0]), wide(g.b[j][0]), acc[i][j], 4, 4, 0, g.as[i], 0, g.bs[j]);
-        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(g.a[i][1]), wide(g.b[j][1]), acc[i][j], 4, 4, 1, g.as[i], 1, g.bs[j]);
+      for (int i = 0; i < 4; ++i) {
+        sa[i] = (int)((unsigned)as[i][s] >> (8 * fq));
+        sb[i] = (int)((unsigned)bs[i][s] >> (8 * fq));
       }
-  };
-  const int k1 = min((sk + 1) * p.kt_per, (p.nb + 7) / 8);
-  for (int kt = sk * p.kt_per + wave; kt < k1; kt += 8) {
-    Group g0, g1;
-    load(g0, kt);
-    load(g1, kt + 4 < k1 ? kt + 4 : -1);
-    multiply(g0);
-    multiply(g1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(a[i][s]), wide(b[j][s]), acc[i][j], 4, 4, 0, sa[i], 0, sb[j]);
+    }
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
@@ -684,9 +681,8 @@ template <typename TO> __global__ __launch_bounds__(256, 1) void mx_dense256_ker
 }
 
 // Float activations against 4-bit weights (serving: the weights are what is read).  A workgroup's four waves own 64 weight rows
-// each (or, where the layer is narrower, share the K groups) x 16 activation rows.  A K group is 512 columns: lane group g takes
-// blocks 4g..4g+3, so a lane reads 64 contiguous bytes of codes and one 32-bit word of scales.  Codes become bf16 with
-// their scale applied (exact: two significant bits) and meet the activations in 16x16x32 bf16 MFMAs, whose k order is the
+// each (or, where the layer is narrower, share the K groups) x 16 activation rows.  A K group is 512 columns: step s of it
+// takes block 4s + (lane >> 4), the row's 16 scale bytes come with one load.  Codes become bf16 with their scale applied (exact: two significant bits) and meet the activations in 16x16x32 bf16 MFMAs, whose k order is the
 // lane's block order on both operands.  The activations of a K group are converted once per workgroup and wait in LDS; fp32 ones
 // are split exactly into three bf16 terms (8 + 8 + 8 bits by truncation) and take three MFMAs: fp32 accuracy, the weights are
 // still read once.
@@ -726,16 +722,14 @@ template <typename TX> __global__ __launch_bounds__(256) void mx_serve_kernel(Mx
   const int gbytes = NX * p.xrows * MXS_ROW;
   for (int kt = k0; kt < k1; kt += kw) {
     // this wave's codes are on their way while the workgroup converts the activations
-    const int b0 = (kt + wk) * 16 + fq * 4;
     const bool mine = kt + wk < k1;
-    i32x4 c[4][4];
-    unsigned sc[4];
+    i32x4 c[4][4], sc[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const unsigned r = (unsigned)(i * 16 + fr);
-      sc[i] = (unsigned)__builtin_amdgcn_raw_buffer_load_b32(wsr, mine ? (int)(r * p.pitch + b0) : (int)MX_OOB, 0, 0);
+      sc[i] = ld16(wsr, mine ? r * p.pitch + (kt + wk) * 16 : MX_OOB);
 #pragma unroll
-      for (int s = 0; s < 4; ++s) c[i][s] = ld16(wr, mine ? r * cp + b0 * 16 + s * 16 : MX_OOB);   // (behind K: times zero)
+      for (int s = 0; s < 4; ++s) c[i][s] = ld16(wr, mine ? r * cp + (kt + wk) * 256 + fq * 16 + s * 64 : MX_OOB);   // (behind K: times zero)
     }
     if (kt > k0) __syncthreads();
     // 8 columns a thread: 64 threads a row and K group
@@ -761,20 +755,20 @@ template <typename TX> __global__ __launch_bounds__(256) void mx_serve_kernel(Mx
     __syncthreads();
     if (!mine) continue;      // (uniform; no weights, and zero times an infinite activation is not zero)
     // (lanes past the rows there are read row 0: a column of the product that nobody stores)
-    const char *xl = lds + wk * gbytes + (fr < p.xrows ? fr : 0) * MXS_ROW + fq * 256;
+    const char *xl = lds + wk * gbytes + (fr < p.xrows ? fr : 0) * MXS_ROW + fq * 64;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       float sf[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const unsigned byte = (sc[i] >> (8 * s)) & 255u;
+        const unsigned byte = ((unsigned)sc[i][s] >> (8 * fq)) & 255u;
         sf[i] = byte == 255u ? __uint_as_float(0x7fc00000u) : mx_scale_f32(byte);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         bf16x8 xb[NX];
 #pragma unroll
-        for (int u = 0; u < NX; ++u) xb[u] = *(const bf16x8 *)(xl + u * p.xrows * MXS_ROW + s * 64 + j * 16);
+        for (int u = 0; u < NX; ++u) xb[u] = *(const bf16x8 *)(xl + u * p.xrows * MXS_ROW + s * 256 + j * 16);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const bf16x8 wv = mx_bf16x8((unsigned)c[i][s][j], sf[i]);
@@ -838,7 +832,7 @@ static void mx_plan(MxDense &p, int x_kind) {
   } else {
     p.nt = (p.N + 63) / 64;
     p.mt = (p.M + 63) / 64;
-    const int groups = (p.nb + 7) / 8;   // two workgroups per CU; a slice has a group for each of the four waves
+    const int groups = p.pitch / 16;     // two workgroups per CU; a slice has a group for each of the four waves
     const int64_t want = 512 / ((int64_t)p.nt * p.mt);
     mx_split(p, groups, want < groups / 4 ? want : groups / 4);
   }
