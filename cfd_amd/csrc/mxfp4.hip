@@ -293,6 +293,7 @@ struct MxDense {
   int kwaves;                         // float activations: waves of a workgroup that share a weight tile
   int xrows;                          //   and activation rows of a tile (<= 16)
   bool big;                           // 256 x 256 tiles
+  bool pairs;                         //   bf16 output: two columns are one aligned word
 };
 
 __device__ __forceinline__ void mx_store(const MxDense &p, int64_t m, int n, float v) {   // one element of the output
@@ -351,7 +352,8 @@ __device__ __forceinline__ i32x4 ld16(__amdgpu_buffer_rsrc_t r, unsigned off) {
 __device__ __forceinline__ i32x8 wide(i32x4 a) { return (i32x8){a[0], a[1], a[2], a[3], 0, 0, 0, 0}; }
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t mx_rsrc(const uint8_t *base, int64_t row0, int rows, int64_t pitch) {
   // tile-relative: rows past the operand fall out of range and read as zero, and no offset needs more than 31 bits
-  return __builtin_amdgcn_make_buffer_rsrc((void *)(base + row0 * pitch), 0, (int)(rows * pitch), 0x00020000);
+  // (the size is uniform, but min() is formed in vector registers: without saying so every load goes through a loop over lanes)
+  return __builtin_amdgcn_make_buffer_rsrc((void *)(base + row0 * pitch), 0, __builtin_amdgcn_readfirstlane((int)(rows * pitch)), 0x00020000);
 }
 
 // tile of a workgroup: each XCD (it has its own L2) gets a contiguous run of them; the tiles of one K slice follow each other
@@ -441,11 +443,8 @@ __global__ __launch_bounds__(256, 2) void mx_dense_kernel(MxDense p) {
 // operands, and 2^-254 is zero in fp32.  Reads past the operand are cut off by the buffer's size, which shrinks as its base advances.
 constexpr int MXT_OPER = 256 * 128, MXT_SCALE = 4 * MXT_OPER, MXT_SCALE_STAGE = 512 * 16;   // W0, W1, X0, X1, scales
 constexpr int MXT_LDS = MXT_SCALE + 2 * MXT_SCALE_STAGE;   // 144 KiB
-constexpr int MXT_ROW = 528;                               // staged output: 512 bytes a row and a pad that spreads the banks
-static_assert(256 * MXT_ROW + 1024 <= MXT_LDS, "the staged output and the bias reuse the stages");
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
-typedef unsigned u32x4a2 __attribute__((ext_vector_type(4), aligned(2)));
 
 __device__ __forceinline__ void mx_dma16(__amdgpu_buffer_rsrc_t r, unsigned voff, unsigned soff, char *dst) {
   __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)dst, 16, (int)voff, (int)soff, 0, 0);
@@ -481,7 +480,8 @@ __device__ __forceinline__ void mx_tile_of(const MxDense &p, int &mt, int &nt, i
   sk = __builtin_amdgcn_readfirstlane(sk);
 }
 
-template <typename TO> __global__ __launch_bounds__(256, 1) void mx_dense256_kernel(MxDense p) {
+enum { MX_PLAIN = 0, MX_LINEAR = 1, MX_SIGMOID = 2 };   // epilogue: the sums; bias and piecewise linear activation; bias and sigmoid
+template <typename TO, int MODE> __global__ __launch_bounds__(256, 1) void mx_dense256_kernel(MxDense p) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave >> 1, wc = wave & 1;
@@ -492,11 +492,11 @@ template <typename TO> __global__ __launch_bounds__(256, 1) void mx_dense256_ker
   const int gbeg = sk * p.kt_per, groups = min(gbeg + p.kt_per, p.pitch / 16) - gbeg;   // of two K tiles = 512 columns
 
   // ---- staging: a wave fills 64 rows of each operand, eight loads of 8 rows; lane -> row lane / 8, source chunk swizzled
-  unsigned voff[8];
+  unsigned vload[8];
 #pragma unroll
   for (int q = 0; q < 8; ++q) {
     const int row = wave * 64 + q * 8 + (lane >> 3);
-    voff[q] = (unsigned)(row * cp + (((lane & 7) ^ ((row >> 1) & 7)) << 4));
+    vload[q] = (unsigned)(row * cp + (((lane & 7) ^ ((row >> 1) & 7)) << 4));
   }
   struct Stream {      // one operand: base of the next K tile, bytes from there to the operand's end, K tiles not issued yet
     const uint8_t *at;
@@ -513,7 +513,7 @@ template <typename TO> __global__ __launch_bounds__(256, 1) void mx_dense256_ker
   Stream w = {p.wc + (int64_t)n0 * cp + (int64_t)gbeg * 256, __builtin_amdgcn_readfirstlane(nr * cp - gbeg * 256), groups * 2};
   Stream x = {p.xc + (int64_t)m0 * cp + (int64_t)gbeg * 256, __builtin_amdgcn_readfirstlane(mr * cp - gbeg * 256), groups * 2};
   char *const dmaw = lds + wave * 8192;
-  auto issue = [&](const Stream &o, int q, int slot) { mx_dma16(o.rsrc(), voff[q], 0, dmaw + slot * MXT_OPER + q * 1024); };
+  auto issue = [&](const Stream &o, int q, int slot) { mx_dma16(o.rsrc(), vload[q], 0, dmaw + slot * MXT_OPER + q * 1024); };
   const __amdgpu_buffer_rsrc_t wsr = mx_rsrc(p.ws, n0, nr, p.pitch), xsr = mx_rsrc(p.xs, m0, mr, p.pitch);
   const unsigned soff = (unsigned)((wave * 64 + lane) * p.pitch);
   unsigned sgrp = (unsigned)gbeg * 16;
@@ -550,7 +550,7 @@ template <typename TO> __global__ __launch_bounds__(256, 1) void mx_dense256_ker
 #define MX_SCALE_W(I, T) as[(I) & 1] = *(const int *)(wsc + ((I) >> 1) * 2048 + ((I) & 1) * 512 + (T) * 8);
 #define MX_READ_X(J, T, S) b[T][J][S] = *(const i32x4 *)(xrd[S] + (T) * MXT_OPER + (J) * 4096);
 #define MX_SCALE_X(J, T) bs[T][J] = *(const int *)(xsc + (J) * 512 + (T) * 8);
-#define MX_MMA(I, T, S, J) acc[I][J] = mx_mma(S, a[(I) & 1][S], b[T][J][S], acc[I][J], as[(I) & 1], bs[T][J]);
+#define MX_MMA(I, T, S, J) acc[I][J] = mx_mma(S, b[T][J][S], a[(I) & 1][S], acc[I][J], bs[T][J], as[(I) & 1]);
 
   issue_scales(0);
 #pragma unroll
@@ -622,62 +622,68 @@ template <typename TO> __global__ __launch_bounds__(256, 1) void mx_dense256_ker
 #undef MX_READ_X
 #undef MX_SCALE_W
 #undef MX_READ_W
-  mx_wait<0>();        // the tail loads must have landed before the stages are reused
-  __syncthreads();
+  mx_wait<0>();        // (the tail loads must not outlive the workgroup's LDS)
 
-  // epilogue: lane holds n = 8q + 4 fh + r (q, r < 4) of fragment row i, pixel row m = fr of fragment j; through LDS, so
-  // that whole 512-byte runs of an output row leave together (fp32: two passes of 128 columns)
-  constexpr int ES = sizeof(TO), NPASS = ES / 2, COLS = 256 / NPASS, EPC = 16 / ES;
-  const bool raw = p.split > 1;
-  TO *const y = raw ? (TO *)p.slab + (int64_t)sk * p.M * p.N : (TO *)p.y;
-  const int64_t ldy = raw ? p.N : p.ldy;
-  const bool sig = p.act == CFD_ACT_SIGMOID && !raw;
-  const float ns = raw || sig ? 1.f : act_neg_scale(p.act, p.slope);
-  float *const sbias = (float *)(lds + 256 * MXT_ROW);
-  sbias[tid] = p.bias && !raw && n0 + tid < p.N ? p.bias[n0 + tid] : 0.f;
-  __syncthreads();
-  auto to_lds = [&](int h, auto with_sigmoid) {   // two copies, chosen once: 256 elements a lane
+  // epilogue straight from the accumulators: lane = column n = fr of fragment i, rows 8q + 4 fh + r of fragment j, so a store covers
+  // 32 consecutive columns of two rows.  bf16: neighbouring lanes swap halves and store two columns of one row each.  (Through
+  // LDS, in whole 512-byte rows, it took 7-10 us of a tile; one wave a SIMD hides no LDS latency.)  Rows and columns that are
+  // not there have offsets past the buffer's size: the stores drop them.
+  TO *const y = p.split > 1 ? (TO *)p.slab + (int64_t)sk * p.M * p.N : (TO *)p.y;
+  const int64_t ldy = p.split > 1 ? p.N : p.ldy;
+  constexpr int ES = sizeof(TO);
+  const int rowb = (int)ldy * ES, nl = wr * 64 + fr, odd = fr & 1;
+  float bias[4];
+  int voff[4];
+  const float ns = act_neg_scale(p.act, p.slope);
+  auto fin = [&](float v, float bv) {
+    if constexpr (MODE == MX_PLAIN) return v;
+    else if constexpr (MODE == MX_LINEAR) return apply_act_linear(v + bv, ns);
+    else return 1.f / (1.f + __expf(-(v + bv)));
+  };
+  auto put = [&](auto pairs) {
 #pragma unroll
-    for (int ii = 0; ii < 4 / NPASS; ++ii) {
-      const int i = h * 2 + ii;
+    for (int i = 0; i < 4; ++i) {
+      const int n = nl + (i >> 1) * 128 + (i & 1) * 32;
+      bias[i] = MODE != MX_PLAIN && p.bias && n < nr ? p.bias[n0 + n] : 0.f;
+      voff[i] = n < nr ? fh * 4 * rowb + n * ES + (decltype(pairs)::value && odd ? rowb - ES : 0) : (int)MX_OOB;
+    }
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int nl = (i >> 1) * 128 + wr * 64 + (i & 1) * 32 + q * 8 + fh * 4;
-        const f32x4 bv = *(const f32x4 *)(sbias + nl);
+    for (int j = 0; j < 4; ++j) {
+      const int m = wc * 128 + j * 32;
+      const int bytes = __builtin_amdgcn_readfirstlane(max(0, min(32, mr - m)) * rowb);
+      const __amdgpu_buffer_rsrc_t yr = __builtin_amdgcn_make_buffer_rsrc((void *)(y + (int64_t)(m0 + m) * ldy + n0), 0, bytes, 0x00020000);
+      int srow = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          TO o[4];
+      for (int q = 0; q < 4; ++q)
 #pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            float v = acc[i][j][q * 4 + r] + bv[r];
-            if constexpr (decltype(with_sigmoid)::value) v = 1.f / (1.f + __expf(-v));
-            o[r] = (TO)apply_act_linear(v, ns);
+        for (int r = 0; r < 4; r += 2) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float v0 = fin(acc[i][j][q * 4 + r], bias[i]), v1 = fin(acc[i][j][q * 4 + r + 1], bias[i]);
+            if constexpr (ES == 4) {
+              __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v0), yr, voff[i] + srow, 0, 0);
+              __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(v1), yr, voff[i] + srow + rowb, 0, 0);
+            } else {
+              const unsigned own = __builtin_bit_cast(unsigned, (bf16x2){(bf16)v0, (bf16)v1});
+              if constexpr (decltype(pairs)::value) {    // odd lanes: {other.hi, own.hi} of the second row, even: {own.lo, other.lo}
+                const unsigned other = (unsigned)__builtin_amdgcn_update_dpp(0, (int)own, 0xB1, 0xf, 0xf, false);
+                __builtin_amdgcn_raw_buffer_store_b32(__builtin_amdgcn_perm(own, other, odd ? 0x07060302u : 0x01000504u), yr,
+                                                      voff[i] + srow, 0, 0);
+              } else {
+                __builtin_amdgcn_raw_buffer_store_b16((unsigned short)own, yr, voff[i] + srow, 0, 0);
+                __builtin_amdgcn_raw_buffer_store_b16((unsigned short)(own >> 16), yr, voff[i] + srow + rowb, 0, 0);
+              }
+            }
           }
-          char *d = lds + (wc * 128 + j * 32 + fr) * MXT_ROW + (nl - h * COLS) * ES;
-          if constexpr (ES == 2) *(bf16x4 *)d = (bf16x4){o[0], o[1], o[2], o[3]};
-          else *(f32x4 *)d = (f32x4){o[0], o[1], o[2], o[3]};
+          srow += r ? 6 * rowb : 2 * rowb;               // (rows 4..7 of eight are the other half's)
+          asm volatile("" : "+s"(srow));                 // (a running sum: all the multiples of rowb at once do not fit the registers)
+          __builtin_amdgcn_sched_barrier(0);
         }
-      }
     }
   };
-#pragma unroll
-  for (int h = 0; h < NPASS; ++h) {
-    if (h) __syncthreads();
-    if (sig) to_lds(h, std::true_type{});
-    else to_lds(h, std::false_type{});
-    __syncthreads();
-    const int c = (lane & 31) * EPC, n = n0 + h * COLS + c;
-#pragma unroll 4
-    for (int it = 0; it < 32; ++it) {
-      const int ml = wave * 64 + it * 2 + (lane >> 5);
-      if (ml >= mr || n >= p.N) continue;
-      const char *src = lds + ml * MXT_ROW + c * ES;
-      TO *dst = y + (int64_t)(m0 + ml) * ldy + n;
-      if (n + EPC <= p.N) *(u32x4a2 *)dst = *(const u32x4a2 *)src;
-      else
-        for (int e = 0; e < p.N - n; ++e) dst[e] = ((const TO *)src)[e];
-    }
-  }
+  if constexpr (ES == 4) put(std::false_type{});
+  else if (p.pairs && nr % 2 == 0) put(std::true_type{});
+  else put(std::false_type{});
 }
 
 // Float activations against 4-bit weights (serving: the weights are what is read).  A workgroup's four waves own 64 weight rows
@@ -814,7 +820,8 @@ static void mx_plan(MxDense &p, int x_kind) {
   const bool serve = x_kind != CFD_MX_X_MXFP4;
   p.nb = (int)mx_blocks(p.K);
   p.pitch = (int)mx_scale_pitch(p.K);
-  p.big = !serve && p.M > 128 && p.N > 128;
+  // measured (us, 256 x 256 tiles | 64 x 64): 1024^2 x 8192 39 | 36, 512 x 1024 x 65536 44 | 84, 256 x 4096^2 35 | 28, 1024^3 19 | 8
+  p.big = !serve && p.M > 128 && p.N > 128 && (double)p.M * p.N * p.K > 1e10;
   if (p.big) {
     p.nt = (p.N + 255) / 256;
     p.mt = (p.M + 255) / 256;
@@ -918,6 +925,7 @@ extern "C" int cfd_mxfp4_dense(const cfd_mxfp4_dense_desc *d, const void *x, con
   if (!d->m || !d->n) return CFD_OK;
   const bool serve = d->x_kind != CFD_MX_X_MXFP4;
   CFD_REQUIRE(x && w_codes && w_scales && y && d->ldy >= d->n, "bad arguments");
+  CFD_REQUIRE(d->ldy <= (1 << 23), "ldy must be at most 8388608");
   CFD_REQUIRE(serve ? d->ldx >= d->k : x_scales != nullptr, "bad activations");
   CFD_REQUIRE((((uintptr_t)w_codes | (uintptr_t)w_scales) & 15) == 0, "weights must be 16-byte aligned");
   CFD_REQUIRE(serve || (((uintptr_t)x | (uintptr_t)x_scales) & 15) == 0, "4-bit activations must be 16-byte aligned");
@@ -927,16 +935,19 @@ extern "C" int cfd_mxfp4_dense(const cfd_mxfp4_dense_desc *d, const void *x, con
   p.xc = (const uint8_t *)x; p.xs = x_scales; p.x = x; p.ldx = d->ldx; p.wc = w_codes; p.ws = w_scales; p.bias = bias;
   p.y = y; p.ldy = d->ldy; p.out_bf16 = d->out_dtype == CFD_BF16; p.act = d->act; p.slope = d->leaky_slope;
   p.slab = (float *)ws;
+  p.pairs = ((uintptr_t)y & 3) == 0 && d->ldy % 2 == 0;
   CFD_REQUIRE(p.split == 1 || ws, "this shape needs a workspace");
   const int64_t blocks = (int64_t)p.mt * p.nt * p.split;
   CFD_REQUIRE(blocks <= 0x7fffffff, "too many tiles");
   hipStream_t st = (hipStream_t)stream;
   if (p.big) {
     const bool b16 = p.out_bf16 && p.split == 1;
-    const void *fn = b16 ? (const void *)mx_dense256_kernel<bf16> : (const void *)mx_dense256_kernel<float>;
-    if (int rc = set_max_lds(fn, MXT_LDS)) return rc;
-    if (b16) hipLaunchKernelGGL(mx_dense256_kernel<bf16>, dim3((unsigned)blocks), dim3(256), MXT_LDS, st, p);
-    else hipLaunchKernelGGL(mx_dense256_kernel<float>, dim3((unsigned)blocks), dim3(256), MXT_LDS, st, p);
+    const int mode = p.split > 1 || (!bias && p.act == CFD_ACT_NONE) ? MX_PLAIN : p.act == CFD_ACT_SIGMOID ? MX_SIGMOID : MX_LINEAR;
+    void (*const fns[2][3])(MxDense) = {{mx_dense256_kernel<float, MX_PLAIN>, mx_dense256_kernel<float, MX_LINEAR>, mx_dense256_kernel<float, MX_SIGMOID>},
+                                        {mx_dense256_kernel<bf16, MX_PLAIN>, mx_dense256_kernel<bf16, MX_LINEAR>, mx_dense256_kernel<bf16, MX_SIGMOID>}};
+    void (*const fn)(MxDense) = fns[b16][mode];
+    if (int rc = set_max_lds((const void *)fn, MXT_LDS)) return rc;
+    hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(256), MXT_LDS, st, p);
   } else if (!serve) {
     hipLaunchKernelGGL(mx_dense_kernel, dim3((unsigned)blocks), dim3(256), 0, st, p);
   } else {
