@@ -820,8 +820,11 @@ static void mx_plan(MxDense &p, int x_kind) {
   const bool serve = x_kind != CFD_MX_X_MXFP4;
   p.nb = (int)mx_blocks(p.K);
   p.pitch = (int)mx_scale_pitch(p.K);
-  // measured (us, 256 x 256 tiles | 64 x 64): 1024^2 x 8192 39 | 36, 512 x 1024 x 65536 44 | 84, 256 x 4096^2 35 | 28, 1024^3 19 | 8
-  p.big = !serve && p.M > 128 && p.N > 128 && (double)p.M * p.N * p.K > 1e10;
+  // 256 x 256 tiles where there are outputs enough to fill the chip without slices of K, or work enough to hide their fixed ~8 us; else
+  // 64 x 64 tiles, which read each operand four times as often.  Measured (us, 256 | 64): 2048^2 x 512 12 | 17, 4000^2 x 100 17 | 51,
+  // 1024^3 11 | 8, 512^2 x 8192 21 | 15, 256 x 4096^2 27 | 27, 1024^2 x 8192 32 | 37, 512 x 1024 x 65536 40 | 83, 136 x 1100 x 4000 19 | 12
+  const double mn = (double)p.M * p.N;
+  p.big = !serve && p.M > 128 && p.N > 128 && (mn >= 3e6 || mn * p.K >= 4e9);
   if (p.big) {
     p.nt = (p.N + 255) / 256;
     p.mt = (p.M + 255) / 256;
