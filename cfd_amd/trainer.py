@@ -109,12 +109,13 @@ class AdamW:
         for p in self.params:
             self.offsets.append(off)
             off += -(-p.numel() // ops.ADAMW_BLOCK) * ops.ADAMW_BLOCK
+        off = max(off, ops.ADAMW_BLOCK)
         z = lambda size, dt: torch.zeros(size, dtype=dt, device=self.device)  # noqa: E731
-        dm, dv = (torch.float32, torch.float32) if state_bits == 32 else (torch.float8_e4m3fn, torch.float8_e5m2)
-        self.m, self.v = z(max(off, 16), torch.uint8 if state_bits == 8 else dm), z(max(off, 16), torch.uint8 if state_bits == 8 else dv)
-        self.m, self.v = self.m.view(dm)[:off], self.v.view(dv)[:off]
-        self.m_scale = z(off // ops.ADAMW_BLOCK, torch.float32) if state_bits == 8 else None
-        self.v_scale = z(off // ops.ADAMW_BLOCK, torch.float32) if state_bits == 8 else None
+        if state_bits == 32:
+            self.m, self.v, self.m_scale, self.v_scale = z(off, torch.float32), z(off, torch.float32), None, None
+        else:
+            self.m, self.v = z(off, torch.uint8).view(torch.float8_e4m3fn), z(off, torch.uint8).view(torch.float8_e5m2)
+            self.m_scale, self.v_scale = z(off // ops.ADAMW_BLOCK, torch.float32), z(off // ops.ADAMW_BLOCK, torch.float32)
         self.t = z(1, torch.int32)
         self._ws = z(32, torch.uint8)
         self._table = (ops.AdamwTensor * n)()

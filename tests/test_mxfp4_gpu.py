@@ -112,9 +112,11 @@ def _close(y, x64, w64, bias, act):
 
 SHAPES = [(1, 1, 32), (1, 1, 1), (5, 3, 31), (16, 16, 128), (64, 64, 256), (65, 63, 257), (100, 130, 1000), (17, 200, 4100),
           (128, 256, 16384), (300, 70, 96), (513, 260, 520), (1, 128, 256), (260, 1, 300), (256, 256, 512), (700, 1030, 2080)]
+#: the 256 x 256 tiles: whole and ragged, odd columns (16-bit stores), a K that ends inside a group, slices of K
+LARGE = [(1800, 1700, 100), (2048, 1536, 512), (1999, 1537, 515), (260, 250, 65536)]
 
 
-@pytest.mark.parametrize("m,n,k", SHAPES)
+@pytest.mark.parametrize("m,n,k", SHAPES + LARGE)
 def test_dense_four_bit_operands(m, n, k):
     from cfd_amd import ops
     x, w = _rnd(m, k, 11, spread=1.0).cuda(), _rnd(n, k, 12, spread=1.0).cuda()
@@ -270,6 +272,28 @@ def test_train_a_wide_dense_head():
                 assert np.abs(_np(t) - p64).max() <= 2.0 ** -21 * (np.abs(p64).max() + 1e-3)
     served = ops.mxfp4_dense(x[:1], ops.mxfp4_quantize(w), bias=bias, act=ops.ACT_RELU)
     _close(served, _np(x[:1]), O.round_trip(_np(w)), bias, 2)
+
+
+def test_matrices_past_32_bits():
+    """more than 2^32 bytes of codes and 2^33 values: the last rows are quantised, decoded and multiplied like a short matrix's"""
+    from cfd_amd import ops
+    rows, k = 66000, 131072
+    x = torch.empty(rows, k, dtype=torch.bfloat16, device="cuda").normal_(generator=torch.Generator(device="cuda").manual_seed(1))
+    q, last = ops.mxfp4_quantize(x), ops.mxfp4_quantize(x[-100:])
+    assert q.codes.numel() > 1 << 32
+    assert torch.equal(q.codes[-100:], last.codes) and torch.equal(q.scales[-100:], last.scales)
+    a = torch.relu(x[:3]).float()
+    del x
+    y, z = ops.mxfp4_dense(a, q), ops.mxfp4_dense(a, last)
+    tol = 64 * 2.0 ** -23 * k ** 0.5 * float(z.abs().max())     # (the K slices differ: other orders of the same fp32 sums)
+    assert (y[:, -100:] - z).abs().max() <= tol
+    aq = ops.mxfp4_quantize(a)
+    assert (ops.mxfp4_dense(aq, q)[:, -100:] - ops.mxfp4_dense(aq, last)).abs().max() <= tol
+    a4 = ops.mxfp4_quantize(a.repeat(100, 1))                   # 300 rows: the 256 x 256 tiles
+    assert (ops.mxfp4_dense(a4, q)[:3, -100:] - ops.mxfp4_dense(aq, last)).abs().max() <= tol
+    del y, z
+    v = ops.mxfp4_dequantize(q, torch.bfloat16)
+    assert torch.equal(v[-100:], ops.mxfp4_dequantize(last, torch.bfloat16))
 
 
 def test_refusals():

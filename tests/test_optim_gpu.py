@@ -240,6 +240,36 @@ def test_grad_norm_extremes():
     assert n[0] == float("inf") and math.isnan(n[1])
 
 
+def test_tensors_past_32_bits():
+    """a tensor of more than 2^31 elements: norm over all of it, and its last elements step like a short tensor's (first step: the
+    parameters do not depend on how the state is rounded)"""
+    from cfd_amd import ops, trainer
+    n = (1 << 31) + 777
+    p, g = torch.zeros(n, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, dtype=torch.bfloat16, device="cuda")
+    tail = torch.randn(5000, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    p[-5000:], g[-5000:] = 0.5, tail
+    want = float(tail.double().square().sum().sqrt())
+    assert abs(float(ops.grad_norm([g], 1.0)[0]) - want) <= 2.0 ** -23 * want
+    q = torch.full((5000,), 0.5, dtype=torch.bfloat16, device="cuda")
+    a, b = trainer.AdamW([p], state_bits=8, **HYPER), trainer.AdamW([q], state_bits=8, **HYPER)
+    a.step([g]), b.step([tail])
+    assert torch.equal(p[-5000:], q) and not p[:-5000].any()
+    lo = n - 4096
+    m = a.m[lo // 256 * 256:].float() * a.m_scale[lo // 256:].repeat_interleave(256)
+    want = 0.1 * g[lo // 256 * 256:].float()
+    m = m[:want.numel()]
+    assert (m - want).abs().max() <= want.abs().max() / 8      # a code step apart at most
+
+
+def test_only_empty_tensors():
+    from cfd_amd import trainer
+    for bits in (32, 8):
+        e = torch.zeros(0, device="cuda")
+        opt = trainer.AdamW([e], state_bits=bits)
+        opt.step([e.clone()])
+        assert int(opt.t) == 1
+
+
 def test_refusals():
     from cfd_amd import _lib, ops, trainer
     c = lambda *s, dt=torch.float32: torch.zeros(*s, dtype=dt, device="cuda")  # noqa: E731
