@@ -170,10 +170,13 @@ constexpr int QT = 128;
 template <typename T> __global__ __launch_bounds__(256) void mx_quant_both_kernel(const T *x, int64_t ldx, int R, int K,
                                                                                    int nb, int pitch, uint8_t *codes,
                                                                                    uint8_t *scales, int nbt, int pitch_t,
-                                                                                   uint8_t *codes_t, uint8_t *scales_t) {
+                                                                                   uint8_t *codes_t, uint8_t *scales_t, int tx) {
   constexpr int W = QT * (int)sizeof(T) / 4;       // words of a tile row
   __shared__ __attribute__((aligned(16))) unsigned tile[QT * W];
-  const int r0 = blockIdx.y * QT, c0 = blockIdx.x * QT;
+  // runs of four neighbouring tiles go to one XCD (workgroups alternate over the eight): the parts of a cache line that they write
+  // meet in one L2 (fp32 4090 x 4102: 26.6 -> 22.6 us; long runs instead set the XCDs a power of two apart: 30 -> 39 us at 4096 x 8192)
+  const int nwg = gridDim.x, wg = blockIdx.x, t = wg < (nwg & ~31) ? (wg & ~31) + (wg & 7) * 4 + ((wg >> 3) & 3) : wg;
+  const int r0 = t / tx * QT, c0 = t % tx * QT;
   const int tid = threadIdx.x, c = (tid & 15) * 8;
   auto put = [&](int i, const Eight<T> &v) {       // eight values of a row into LDS, coded along the row
     const int r = i * 16 + (tid >> 4);
@@ -877,13 +880,15 @@ extern "C" int cfd_mxfp4_quantize(const void *x, int64_t ldx, int dtype, int64_t
   } else {
     if (int rc = mx_check(cols, 0, rows)) return rc;   // the rows are the other orientation's columns
     const int nbt = (int)mx_blocks(rows), pitch_t = (int)mx_scale_pitch(rows);
-    const dim3 grid((unsigned)((cols + QT - 1) / QT), (unsigned)((rows + QT - 1) / QT));
+    const int64_t tx = (cols + QT - 1) / QT, blocks = tx * ((rows + QT - 1) / QT);
+    CFD_REQUIRE(blocks <= 0x7fffffff, "too many elements");
+    const dim3 grid((unsigned)blocks);
     if (dtype == CFD_BF16)
       hipLaunchKernelGGL(mx_quant_both_kernel<bf16>, grid, dim3(256), 0, st, (const bf16 *)x, ldx, (int)rows, (int)cols, nb,
-                         pitch, codes, scales, nbt, pitch_t, codes_t, scales_t);
+                         pitch, codes, scales, nbt, pitch_t, codes_t, scales_t, (int)tx);
     else
       hipLaunchKernelGGL(mx_quant_both_kernel<float>, grid, dim3(256), 0, st, (const float *)x, ldx, (int)rows, (int)cols, nb,
-                         pitch, codes, scales, nbt, pitch_t, codes_t, scales_t);
+                         pitch, codes, scales, nbt, pitch_t, codes_t, scales_t, (int)tx);
   }
   CFD_LAUNCH_CHECK();
   return CFD_OK;
