@@ -308,3 +308,41 @@ def test_refusals():
     with pytest.raises(RuntimeError):
         opt.step([c(8)])
     assert int(opt.t) == 0
+
+
+def test_regressor_step_on_its_parameter_store():
+    """the regressor's own forward and backward, its parameters and gradients as views of the flat buffers, clipped AdamW with an 8-bit
+    state writing master and compute copy, then the trained wide layer in 4 bits beside the bf16 one"""
+    from oracle import mxfp4 as OM
+    from cfd_amd import nets, ops, trainer
+    net = nets.CnnRegressor((16, 64, 1), dtype=torch.bfloat16, seed=5)
+    P = net.params
+    P.enable_training()
+    names = [n for n, s in P.specs.items() if s.kind != "stat"]
+    wd = [0.004 if n.endswith("kernel") else 0.0 for n in names]
+    opt = trainer.AdamW([P.m(n) for n in names], copies=[P.c(n) for n in names], weight_decay=wd, state_bits=8, **HYPER)
+    gen = torch.Generator().manual_seed(2)
+    x, target = torch.randn(4, 16, 64, 1, generator=gen).cuda(), torch.randn(4, 1, generator=gen).cuda()
+    for step in range(3):
+        P.zero_grad()
+        y = net.forward(x, training=True, seed=step)
+        dy, loss = torch.empty_like(y), torch.zeros(1, device="cuda")
+        ops.field_loss(y, target, ops.MSE, loss, dout=dy)
+        net.backward(dy, x, seed=step)
+        grads = [P.g(n) for n in names]
+        norm = ops.grad_norm(grads, 0.1)
+        want = O.grad_norm([_f64(g) for g in grads], 0.1)
+        assert abs(float(norm[0]) - want[0]) <= 2.0 ** -23 * want[0]
+        _check_step(opt, grads, float(norm[1]), HYPER["lr"], wd)
+        P.refresh_transposed()
+    feats = torch.relu(torch.randn(3, P.c("fc1.kernel").shape[1], generator=gen)).to(torch.bfloat16).cuda()
+    w4 = ops.mxfp4_quantize(P.c("fc1.kernel"))
+    y4 = ops.mxfp4_dense(feats, w4, bias=P.m("fc1.bias"), act=ops.ACT_RELU, out_dtype=torch.float32)
+    w64 = OM.round_trip(_f64(P.c("fc1.kernel")))
+    ref = np.maximum(_f64(feats) @ w64.T + _f64(P.m("fc1.bias")), 0)
+    mag = _f64(feats) @ np.abs(w64).T + 1.0
+    assert (np.abs(_f64(y4) - ref) <= (w64.shape[1] / 32 + 64) * 2.0 ** -23 * mag).all()
+    y16 = ops.conv_forward(feats, P.c("fc1.kernel"), P.m("fc1.bias"), ops.DENSE, 256, act=ops.ACT_RELU, out_dtype=torch.float32)
+    # the two layers differ by what the weights lost, and by fp32 sums
+    off = _f64(feats) @ np.abs(w64 - _f64(P.c("fc1.kernel"))).T
+    assert (np.abs(_f64(y4) - _f64(y16)) <= off * 1.01 + 8192 / 32 * 2.0 ** -23 * mag).all()
