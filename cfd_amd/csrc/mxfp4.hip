@@ -441,7 +441,8 @@ __global__ __launch_bounds__(256, 2) void mx_dense_kernel(MxDense p) {
 //   * scales: 16 bytes a row cover two K tiles (8 KiB, two stages, two LDS-DMA loads per wave every second K tile);
 //   * a wave holds its 128 activation rows of the K tile in registers and walks its weight rows 32 at a time: 16 MFMAs, between which
 //     it reads the next 32 weight rows and a part of the next K tile's activations.  Two barriers per K tile: behind the first
-//     the activations' other stage is free, behind the second the weights', and each is refilled a whole K tile ahead of its use.
+//     the activations' other stage is free, behind the second the weights', and each is refilled a whole K tile ahead of its use, one
+//     load every four MFMAs (in bursts of eight: 3 % slower at 4096 x 4096 x 8192).
 // The K range goes in groups of two K tiles; codes behind the last column need no mask: their scale bytes are zero on both
 // operands, and 2^-254 is zero in fp32.  Reads past the operand are cut off by the buffer's size, which shrinks as its base advances.
 constexpr int MXT_OPER = 256 * 128, MXT_SCALE = 4 * MXT_OPER, MXT_SCALE_STAGE = 512 * 16;   // W0, W1, X0, X1, scales
@@ -462,11 +463,11 @@ __device__ __forceinline__ f32x16 mx_mma(int s, i32x4 a, i32x4 b, f32x16 c, int 
   }
 }
 template <int N> __device__ __forceinline__ void mx_wait() {
-  static_assert(N == 0 || N == 8 || N == 10 || N == 18, "counts that the schedule uses");
+  static_assert(N == 0 || N == 8 || N == 10 || N == 13, "counts that the schedule uses");
   if constexpr (N == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
   else if constexpr (N == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
   else if constexpr (N == 10) asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
-  else asm volatile("s_waitcnt vmcnt(18)" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(13)" ::: "memory");
 }
 
 // tile of a workgroup: each XCD gets a contiguous run of tiles (it has its own L2), and runs walk 8 m tiles before the next
@@ -565,9 +566,9 @@ template <typename TO, int MODE> __global__ __launch_bounds__(256, 1) void mx_de
   for (int q = 0; q < 8; ++q) issue(x, q, 3);
   issue_scales(MXT_SCALE_STAGE);
 #pragma unroll
-  for (int q = 0; q < 8; ++q) issue(w, q, 1);
-  x.advance(); w.advance();
-  mx_wait<18>();
+  for (int q = 0; q < 3; ++q) issue(w, q, 1);      // (the other five in the loop)
+  x.advance();
+  mx_wait<13>();
   __builtin_amdgcn_s_barrier();
 #pragma unroll
   for (int s = 0; s < 4; ++s) {
@@ -595,7 +596,7 @@ template <typename TO, int MODE> __global__ __launch_bounds__(256, 1) void mx_de
           __builtin_amdgcn_s_barrier();                                                                             \
           if constexpr ((T) == 1) xsc = flip(xsc);                                                                  \
         }                                                                                                           \
-        if (i == 1 && y >= 8) issue(x, y - 8, 2 + (T));                                                             \
+        if ((i == 1 || i == 2) && (y & 3) == 1) issue(x, (i - 1) * 4 + (y >> 2), 2 + (T));                          \
         if (i == 1 && y >= 8 && y < 12) { MX_READ_X(0, 1 - (T), y - 8) }                                            \
         if (i == 1 && y >= 12) { MX_SCALE_X(y - 12, 1 - (T)) }                                                      \
         if (i == 2 && y >= 6 && y < 14) { MX_READ_X(1 + ((y - 6) >> 2), 1 - (T), (y - 6) & 3) }                     \
@@ -607,12 +608,14 @@ template <typename TO, int MODE> __global__ __launch_bounds__(256, 1) void mx_de
         }                                                                                                           \
         if (i == 3 && y >= 3 && y < 7) { MX_READ_W(0, 1 - (T), y - 3) }                                             \
         if (i == 3 && y == 7) { MX_SCALE_W(0, 1 - (T)) }                                                            \
-        if (i == 3 && y >= 4 && y < 12) issue(w, y - 4, T);                                                         \
+        if (i == 3 && (y & 3) == 1 && y > 1) issue(w, (y >> 2) - 1, T);                                             \
+        if (i == 0 && (y & 1) && y < 10) issue(w, 3 + (y >> 1), 1 - (T));                                           \
+        if (i == 0 && y == 10) w.advance();                                                                         \
         if (i == 3 && y >= 8 && y < 12) { MX_READ_X(3, 1 - (T), y - 8) }                                            \
         __builtin_amdgcn_sched_barrier(0);                                                                          \
       }                                                                                                             \
     }                                                                                                               \
-    x.advance(); w.advance();                                                                                       \
+    x.advance();                                                                                                    \
   }
   for (int g = 0; g < groups; ++g) {
     MX_KTILE(0)
