@@ -8,6 +8,7 @@
 // a spacing at its block's top (the plain floor would clip a block's largest values by up to a quarter); codes round to
 // nearest even.  A block with an infinity or NaN gets the scale 0xFF: the whole block reads as NaN.
 #include "common.h"
+#include "igemm256.h"
 #include <type_traits>
 
 namespace cfd {
@@ -17,6 +18,14 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef __bf16 bf16x8a2 __attribute__((ext_vector_type(8), aligned(2)));
 typedef __bf16 bf16x4a2 __attribute__((ext_vector_type(4), aligned(2)));
+
+// threads of a launch per matrix row: a 64-bit division by it would be most of a streaming kernel's instructions
+struct FastDiv {
+  unsigned d, c[3];
+  explicit FastDiv(unsigned v) : d(v) { fastdiv_make(v, c); }
+  __device__ __forceinline__ unsigned div(unsigned n) const { return (unsigned)fastdiv((int)n, c); }
+};
+constexpr int64_t MX_GRID = 0xffffff;   // workgroups of 256 threads, under 2^32 threads in all
 
 static inline int64_t mx_blocks(int64_t k) { return (k + 31) / 32; }
 static inline int64_t mx_scale_pitch(int64_t k) { return (mx_blocks(k) + 15) / 16 * 16; }
@@ -149,12 +158,11 @@ __device__ __forceinline__ unsigned quad_bytes(unsigned byte) {   // the same ov
 // lanes hold four whole scale bytes.
 template <typename T> __global__ __launch_bounds__(256) void mx_quant_rows_kernel(const T *x, int64_t ldx, int64_t rows, int K,
                                                                                    int nb, int pitch, uint8_t *codes,
-                                                                                   uint8_t *scales) {
-  const int64_t G = (int64_t)((nb + 3) / 4) * 16, total = rows * G;
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t >= total) return;                 // (whole rows of 16 lanes: G is a multiple of 16)
-  const int64_t row = t / G;
-  const int grp = (int)(t - row * G);
+                                                                                   uint8_t *scales, FastDiv G) {
+  const unsigned t = blockIdx.x * 256 + threadIdx.x;       // (the host keeps the grid under 2^32 threads)
+  const int64_t row = G.div(t);
+  if (row >= rows) return;                // (whole rows of 16 lanes: G is a multiple of 16)
+  const int grp = (int)(t - (unsigned)row * G.d);
   Eight<T> v;
   v.load(x + row * ldx + (int64_t)grp * 8, K - grp * 8);
   const unsigned byte = mx_scale_byte(quad_umax(amax8(v.get())));
@@ -239,43 +247,43 @@ template <typename T> __global__ __launch_bounds__(256) void mx_quant_both_kerne
   }
 }
 
-// codes -> values: a lane reads eight codes and writes 16 (bf16) or 32 (fp32) bytes
+__device__ __forceinline__ bf16x8 mx_bf16x8(unsigned c, float s) {     // eight codes times their scale
+  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1);
+  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2), e = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3);
+  return (bf16x8){a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1]};
+}
+__device__ __forceinline__ float mx_scale_or_nan(unsigned byte) { return byte == 255u ? __uint_as_float(0x7fc00000u) : mx_scale_f32(byte); }
+
+// codes -> values (exact, or an overflow to infinity at the top of the scale's range): a lane reads eight codes and writes 16 (bf16)
+// or 32 (fp32) bytes
 template <typename T> __global__ __launch_bounds__(256) void mx_dequant_kernel(const uint8_t *codes, const uint8_t *scales,
                                                                                 int64_t rows, int K, int nb, int pitch, T *y,
-                                                                                int64_t ldy) {
-  const int64_t G = (int64_t)nb * 4, total = rows * G;
-  const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t >= total) return;
-  const int64_t row = t / G;
-  const int grp = (int)(t - row * G), left = K - grp * 8;
+                                                                                int64_t ldy, FastDiv G) {
+  const unsigned t = blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = G.div(t);
+  if (row >= rows) return;
+  const int grp = (int)(t - (unsigned)row * G.d), left = K - grp * 8;
   const unsigned c = *(const unsigned *)(codes + row * nb * 16 + (int64_t)grp * 4);
-  const unsigned byte = scales[row * pitch + (grp >> 2)];
-  const float s = byte == 255u ? __uint_as_float(0x7fc00000u) : mx_scale_f32(byte);
-  float v[8];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const f32x2 p = i == 0   ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 0)
-                    : i == 1 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 1)
-                    : i == 2 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 2)
-                             : __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 3);
-    v[2 * i] = p[0] * s;          // exact, or an overflow to infinity at the top of the scale's range
-    v[2 * i + 1] = p[1] * s;
-  }
+  const float s = mx_scale_or_nan(scales[row * pitch + (grp >> 2)]);
   T *o = y + row * ldy + (int64_t)grp * 8;
-  if (left >= 8) {
-    if constexpr (sizeof(T) == 2) {
-      bf16x8a2 w;
+  if constexpr (sizeof(T) == 2) {
+    const bf16x8 v = mx_bf16x8(c, s);
+    if (left >= 8) *(bf16x8a2 *)o = v;
+    else
 #pragma unroll
-      for (int i = 0; i < 8; ++i) w[i] = (bf16)v[i];
-      *(bf16x8a2 *)o = w;
-    } else {
-      *(f32x4a4 *)o = (f32x4){v[0], v[1], v[2], v[3]};
-      *(f32x4a4 *)(o + 4) = (f32x4){v[4], v[5], v[6], v[7]};
-    }
+      for (int i = 0; i < 8; ++i)
+        if (i < left) o[i] = v[i];
   } else {
+    const f32x2 p[4] = {__builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 0), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 1),
+                        __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 2), __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, 1.f, 3)};
+    if (left >= 8) {
+      *(f32x4a4 *)o = (f32x4){p[0][0] * s, p[0][1] * s, p[1][0] * s, p[1][1] * s};
+      *(f32x4a4 *)(o + 4) = (f32x4){p[2][0] * s, p[2][1] * s, p[3][0] * s, p[3][1] * s};
+    } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (i < left) o[i] = (T)v[i];
+      for (int i = 0; i < 8; ++i)
+        if (i < left) o[i] = p[i >> 1][i & 1] * s;
+    }
   }
 }
 
@@ -711,12 +719,6 @@ __device__ __forceinline__ Split3 split3(float x) {
   r.t[0] = (bf16)h; r.t[1] = (bf16)m; r.t[2] = (bf16)(d - m);
   return r;
 }
-__device__ __forceinline__ bf16x8 mx_bf16x8(unsigned c, float s) {
-  const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 0), b = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 1);
-  const bf16x2 d = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 2), e = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, 3);
-  return (bf16x8){a[0], a[1], b[0], b[1], d[0], d[1], e[0], e[1]};
-}
-
 constexpr int MXS_ROW = 1024 + 16;      // bytes of one activation row's K group in LDS: 512 bf16 and a pad
 template <typename TX> __global__ __launch_bounds__(256) void mx_serve_kernel(MxDense p) {
   constexpr int NX = sizeof(TX) == 4 ? 3 : 1;
@@ -773,8 +775,7 @@ template <typename TX> __global__ __launch_bounds__(256) void mx_serve_kernel(Mx
       float sf[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const unsigned byte = ((unsigned)sc[i][s] >> (8 * fq)) & 255u;
-        sf[i] = byte == 255u ? __uint_as_float(0x7fc00000u) : mx_scale_f32(byte);
+        sf[i] = mx_scale_or_nan(((unsigned)sc[i][s] >> (8 * fq)) & 255u);
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -868,23 +869,25 @@ extern "C" int cfd_mxfp4_quantize(const void *x, int64_t ldx, int dtype, int64_t
   CFD_REQUIRE((codes != nullptr) == (scales != nullptr) && (codes_t != nullptr) == (scales_t != nullptr) && (codes || codes_t),
               "codes come with scales, in one orientation at least");
   CFD_REQUIRE(x && ldx >= cols, "bad arguments");
-  CFD_REQUIRE(((uintptr_t)codes & 15) == 0 && ((uintptr_t)codes_t & 15) == 0, "codes must be 16-byte aligned");
+  CFD_REQUIRE((((uintptr_t)codes | (uintptr_t)scales | (uintptr_t)codes_t | (uintptr_t)scales_t) & 15) == 0,
+              "codes and scales must be 16-byte aligned");
   hipStream_t st = (hipStream_t)stream;
   const int nb = (int)mx_blocks(cols), pitch = (int)mx_scale_pitch(cols);
   if (!codes_t) {
-    const int64_t blocks = (rows * ((nb + 3) / 4 * 16) + 255) / 256;
-    CFD_REQUIRE(blocks <= 0x7fffffff, "too many elements");
+    const FastDiv G((unsigned)((nb + 3) / 4 * 16));
+    const int64_t blocks = (rows * G.d + 255) / 256;
+    CFD_REQUIRE(blocks <= MX_GRID, "too many elements");
     if (dtype == CFD_BF16)
       hipLaunchKernelGGL(mx_quant_rows_kernel<bf16>, dim3((unsigned)blocks), dim3(256), 0, st, (const bf16 *)x, ldx, rows,
-                         (int)cols, nb, pitch, codes, scales);
+                         (int)cols, nb, pitch, codes, scales, G);
     else
       hipLaunchKernelGGL(mx_quant_rows_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, st, (const float *)x, ldx, rows,
-                         (int)cols, nb, pitch, codes, scales);
+                         (int)cols, nb, pitch, codes, scales, G);
   } else {
     if (int rc = mx_check(cols, 0, rows)) return rc;   // the rows are the other orientation's columns
     const int nbt = (int)mx_blocks(rows), pitch_t = (int)mx_scale_pitch(rows);
     const int64_t tx = (cols + QT - 1) / QT, blocks = tx * ((rows + QT - 1) / QT);
-    CFD_REQUIRE(blocks <= 0x7fffffff, "too many elements");
+    CFD_REQUIRE(blocks <= MX_GRID, "too many elements");
     const dim3 grid((unsigned)blocks);
     if (dtype == CFD_BF16)
       hipLaunchKernelGGL(mx_quant_both_kernel<bf16>, grid, dim3(256), 0, st, (const bf16 *)x, ldx, (int)rows, (int)cols, nb,
@@ -903,15 +906,17 @@ extern "C" int cfd_mxfp4_dequantize(const uint8_t *codes, const uint8_t *scales,
   CFD_REQUIRE(dtype == CFD_F32 || dtype == CFD_BF16, "bad dtype");
   if (rows == 0) return CFD_OK;
   CFD_REQUIRE(codes && scales && y && ldy >= cols, "bad arguments");
+  CFD_REQUIRE((((uintptr_t)codes | (uintptr_t)scales) & 15) == 0, "codes and scales must be 16-byte aligned");
   const int nb = (int)mx_blocks(cols), pitch = (int)mx_scale_pitch(cols);
-  const int64_t blocks = (rows * nb * 4 + 255) / 256;
-  CFD_REQUIRE(blocks <= 0x7fffffff, "too many elements");
+  const FastDiv G((unsigned)(nb * 4));
+  const int64_t blocks = (rows * G.d + 255) / 256;
+  CFD_REQUIRE(blocks <= MX_GRID, "too many elements");
   if (dtype == CFD_BF16)
     hipLaunchKernelGGL(mx_dequant_kernel<bf16>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, codes, scales, rows,
-                       (int)cols, nb, pitch, (bf16 *)y, ldy);
+                       (int)cols, nb, pitch, (bf16 *)y, ldy, G);
   else
     hipLaunchKernelGGL(mx_dequant_kernel<float>, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, codes, scales, rows,
-                       (int)cols, nb, pitch, (float *)y, ldy);
+                       (int)cols, nb, pitch, (float *)y, ldy, G);
   CFD_LAUNCH_CHECK();
   return CFD_OK;
 }
@@ -949,7 +954,7 @@ extern "C" int cfd_mxfp4_dense(const cfd_mxfp4_dense_desc *d, const void *x, con
   p.pairs = ((uintptr_t)y & 3) == 0 && d->ldy % 2 == 0;
   CFD_REQUIRE(p.split == 1 || ws, "this shape needs a workspace");
   const int64_t blocks = (int64_t)p.mt * p.nt * p.split;
-  CFD_REQUIRE(blocks <= 0x7fffffff, "too many tiles");
+  CFD_REQUIRE(blocks <= MX_GRID, "too many tiles");
   hipStream_t st = (hipStream_t)stream;
   if (p.big) {
     const bool b16 = p.out_bf16 && p.split == 1;
@@ -973,7 +978,7 @@ extern "C" int cfd_mxfp4_dense(const cfd_mxfp4_dense_desc *d, const void *x, con
   CFD_LAUNCH_CHECK();
   if (p.split > 1) {
     const int64_t b = (d->m * d->n + 63) / 64;
-    CFD_REQUIRE(b <= 0x7fffffff, "too many outputs");
+    CFD_REQUIRE(b <= MX_GRID, "too many outputs");
     hipLaunchKernelGGL(mx_split_sum_kernel, dim3((unsigned)b), dim3(256), 0, st, p);
     CFD_LAUNCH_CHECK();
   }

@@ -330,7 +330,7 @@ extern "C" int cfd_grad_norm(const void *const *g, const int64_t *n, int count, 
   CFD_REQUIRE(max_norm > 0.f, "max_norm must be positive");
   for (int i = 0; i < count; ++i) CFD_REQUIRE(n[i] >= 0 && (g[i] || !n[i]), "tensor %d: NULL pointer or negative length", i);
   const int64_t chunk = norm_chunk(n, count), blocks = norm_blocks(n, count, chunk);
-  CFD_REQUIRE(blocks <= 0x7fffffff, "too many elements");
+  CFD_REQUIRE(blocks <= 0xffffff, "too many elements");
   hipStream_t st = (hipStream_t)stream;
   int64_t done = 0;
   for (int i = 0; i < count;) {
@@ -369,7 +369,7 @@ extern "C" int cfd_adamw_step(const cfd_adamw_tensor *t, int count, const cfd_ad
     CFD_REQUIRE(!t[i].copy || d->p_dtype == CFD_F32, "tensor %d: a bf16 copy needs an fp32 parameter", i);
     blocks += (t[i].n + OPT_CHUNK - 1) / OPT_CHUNK;
   }
-  CFD_REQUIRE(blocks <= 0x7fffffff, "too many elements");
+  CFD_REQUIRE(blocks <= 0xffffff, "too many elements");
   hipStream_t st = (hipStream_t)stream;
   AdamwHyper *h = (AdamwHyper *)ws;
   hipLaunchKernelGGL(adamw_begin_kernel, dim3(1), dim3(1), 0, st, step, h, lr_device, d->lr, grad_scale, d->beta1, d->beta2, d->seed);
