@@ -302,7 +302,7 @@ struct MxDense {
   int out_bf16, act;
   float slope;
   int kwaves;                         // float activations: waves of a workgroup that share a weight tile
-  int xrows;                          //   and activation rows of a tile (<= 16)
+  int xrows;                          //   and activation rows of a tile
   bool big;                           // 256 x 256 tiles
   bool pairs;                         //   bf16 output: two columns are one aligned word
 };
@@ -378,14 +378,32 @@ __device__ __forceinline__ void mx_small_tile(const MxDense &p, int &mt, int &nt
   nt = __builtin_amdgcn_readfirstlane(nt);
 }
 
+// LDS-DMA: lane l's 16 bytes land at dst + 16 l.  Matrix fragments come this way rather than straight into registers: their lanes
+// want 16 different rows, and neighbouring lanes in different rows make a request each (77 a load instruction: 26 of the 26 us at
+// 128 x 256 x 262144), while here neighbouring lanes take neighbouring 16 bytes.
+__device__ __forceinline__ void mx_dma16(__amdgpu_buffer_rsrc_t r, unsigned voff, unsigned soff, char *dst) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)dst, 16, (int)voff, (int)soff, 0, 0);
+}
+template <int N> __device__ __forceinline__ void mx_wait() {   // until at most N vector-memory operations are in flight
+  static_assert(N == 0 || N == 8 || N == 10 || N == 13 || N == 16 || N == 18, "counts that the schedules use");
+  if constexpr (N == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  else if constexpr (N == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
+  else if constexpr (N == 10) asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
+  else if constexpr (N == 13) asm volatile("s_waitcnt vmcnt(13)" ::: "memory");
+  else if constexpr (N == 16) asm volatile("s_waitcnt vmcnt(16)" ::: "memory");
+  else asm volatile("s_waitcnt vmcnt(18)" ::: "memory");
+}
+__device__ __forceinline__ void mx_wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 // Both operands in 4 bits, small or long products (bound by reading them): a workgroup owns 64 (m) x 64 (n), its four waves take
-// K groups of 512 columns in turn and join in LDS.  Fragments go from global memory straight into the scaled MFMA
-// (16x16x128: lane = row l & 15, block l >> 4, its scale byte its own); step s of a group takes block 4s + (l >> 4), so a load
-// instruction covers 64 contiguous bytes of 16 rows.  The 16 scale bytes of a row's group come with one load (a load for each
-// step cost as much as the codes: 30 -> 24 us at 128 x 256 x 262144 without them); a lane shifts its byte down.
-// Codes behind the last column (the next row's) need no mask: their scale bytes are zero on both operands, 2^-254 is zero in fp32.
-__global__ __launch_bounds__(256, 2) void mx_dense_kernel(MxDense p) {
-  __shared__ f32x4 part[4][16][64];
+// K groups of 512 columns in turn and join in LDS.  Every wave streams for itself, without barriers: a half group (256 columns, 8 KiB
+// of each operand) in two stages, the 16 scale bytes a row of a group in two more; the next half is under way while this one
+// multiplies.  16x16x128 scaled MFMA: lane = row l & 15, step s takes block 4s + (l >> 4), a lane shifts its scale byte down.
+// Chunks are XOR-ed with bits 1-3 of the row (see the 256 x 256 kernel).  Codes behind the last column (the next row's) need no
+// mask: their scale bytes are zero on both operands, 2^-254 is zero in fp32.
+constexpr int MXD_OPER = 64 * 128, MXD_STAGE = 2 * MXD_OPER, MXD_WAVE = 2 * MXD_STAGE + 2 * 2048, MXD_LDS = 4 * MXD_WAVE;   // 144 KiB
+__global__ __launch_bounds__(256, 1) void mx_dense_kernel(MxDense p) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
   int mt, nt, sk;
   mx_small_tile(p, mt, nt, sk);
   const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
@@ -394,36 +412,71 @@ __global__ __launch_bounds__(256, 2) void mx_dense_kernel(MxDense p) {
   const int mr = min(64, p.M - m0), nr = min(64, p.N - n0);
   const __amdgpu_buffer_rsrc_t xr = mx_rsrc(p.xc, m0, mr, cp), wr = mx_rsrc(p.wc, n0, nr, cp);
   const __amdgpu_buffer_rsrc_t xsr = mx_rsrc(p.xs, m0, mr, p.pitch), wsr = mx_rsrc(p.ws, n0, nr, p.pitch);
-  f32x4 acc[4][4] = {};
-  const int k1 = min((sk + 1) * p.kt_per, p.pitch / 16);
-  for (int kt = sk * p.kt_per + wave; kt < k1; kt += 4) {
-    i32x4 a[4][4], b[4][4], as[4], bs[4];
+  char *const my = lds + wave * MXD_WAVE;
+  const unsigned lrow = lane >> 3;
+  auto issue = [&](int kt, int half) {            // 16 loads: 8 rows of 128 bytes each (rows past the operand read as zero)
+    const unsigned at = (unsigned)kt * 256 + half * 128;
+    char *dst = my + half * MXD_STAGE;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const unsigned row = (unsigned)(i * 16 + fr);    // (rows past the operand lie past its size and read as zero)
-      as[i] = ld16(wsr, row * p.pitch + kt * 16);
-      bs[i] = ld16(xsr, row * p.pitch + kt * 16);
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        a[i][s] = ld16(wr, row * cp + kt * 256 + fq * 16 + s * 64);
-        b[i][s] = ld16(xr, row * cp + kt * 256 + fq * 16 + s * 64);
-      }
+    for (int q = 0; q < 8; ++q) {
+      const unsigned row = q * 8 + lrow, off = row * cp + (((lane & 7) ^ ((row >> 1) & 7)) << 4) + at;
+      mx_dma16(wr, off, 0, dst + q * 1024);
+      mx_dma16(xr, off, 0, dst + MXD_OPER + q * 1024);
     }
+  };
+  auto issue_scales = [&](int kt, int stage) {
+    const unsigned off = (unsigned)(lane * p.pitch + kt * 16);
+    mx_dma16(wsr, off, 0, my + 2 * MXD_STAGE + stage);
+    mx_dma16(xsr, off, 0, my + 2 * MXD_STAGE + stage + 1024);
+  };
+  f32x4 acc[4][4] = {};
+  auto multiply = [&](int half, int stage, auto next) {     // `next` starts the loads that may overwrite what has been read
+    i32x4 a[4][2], b[4][2];
+    int sa[4][2], sb[4][2];
+    const char *src = my + half * MXD_STAGE + fr * 128, *sc = my + 2 * MXD_STAGE + stage + fr * 16 + half * 8;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      int sa[4], sb[4];
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int chunk = ((4 * s + fq) ^ ((fr >> 1) & 7)) << 4;
+        a[i][s] = *(const i32x4 *)(src + i * 2048 + chunk);
+        b[i][s] = *(const i32x4 *)(src + MXD_OPER + i * 2048 + chunk);
+        sa[i][s] = *(const int *)(sc + i * 256 + s * 4);
+        sb[i][s] = *(const int *)(sc + 1024 + i * 256 + s * 4);
+      }
+    mx_wait_lds();
+    next();
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        sa[i] = (int)((unsigned)as[i][s] >> (8 * fq));
-        sb[i] = (int)((unsigned)bs[i][s] >> (8 * fq));
+        sa[i][s] = (int)((unsigned)sa[i][s] >> (8 * fq));
+        sb[i][s] = (int)((unsigned)sb[i][s] >> (8 * fq));
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(a[i][s]), wide(b[j][s]), acc[i][j], 4, 4, 0, sa[i], 0, sb[j]);
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wide(a[i][s]), wide(b[j][s]), acc[i][j], 4, 4, 0, sa[i][s], 0, sb[j][s]);
     }
+  };
+  const int k1 = min((sk + 1) * p.kt_per, p.pitch / 16);
+  int kt = sk * p.kt_per + wave, stage = 0;
+  if (kt < k1) {
+    issue_scales(kt, 0);
+    issue(kt, 0);
+    issue(kt, 1);
+    for (; kt < k1; kt += 4) {     // (behind the slice's end the next group is loaded all the same: the counts stay, nobody reads it)
+      mx_wait<16>();               // this group's scales and first half; its second half is in flight
+      multiply(0, stage, [&] { issue_scales(kt + 4, stage ^ 2048); issue(kt + 4, 0); });
+      mx_wait<18>();               // the second half; the next group's scales and first half are in flight
+      multiply(1, stage, [&] { issue(kt + 4, 1); });
+      stage ^= 2048;
+    }
+    mx_wait<0>();                  // (the tail loads must not land in what follows)
   }
+  __syncthreads();
+  f32x4 (*const part)[16][64] = (f32x4 (*)[16][64])lds;
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -458,9 +511,6 @@ constexpr int MXT_LDS = MXT_SCALE + 2 * MXT_SCALE_STAGE;   // 144 KiB
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
-__device__ __forceinline__ void mx_dma16(__amdgpu_buffer_rsrc_t r, unsigned voff, unsigned soff, char *dst) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (__attribute__((address_space(3))) void *)dst, 16, (int)voff, (int)soff, 0, 0);
-}
 // one 32x32x64 step; the scale byte is an immediate of the instruction (s is a constant after unrolling)
 __device__ __forceinline__ f32x16 mx_mma(int s, i32x4 a, i32x4 b, f32x16 c, int as, int bs) {
   switch (s) {
@@ -470,14 +520,6 @@ __device__ __forceinline__ f32x16 mx_mma(int s, i32x4 a, i32x4 b, f32x16 c, int 
     default: return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a), wide(b), c, 4, 4, 3, as, 3, bs);
   }
 }
-template <int N> __device__ __forceinline__ void mx_wait() {
-  static_assert(N == 0 || N == 8 || N == 10 || N == 13, "counts that the schedule uses");
-  if constexpr (N == 0) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  else if constexpr (N == 8) asm volatile("s_waitcnt vmcnt(8)" ::: "memory");
-  else if constexpr (N == 10) asm volatile("s_waitcnt vmcnt(10)" ::: "memory");
-  else asm volatile("s_waitcnt vmcnt(13)" ::: "memory");
-}
-
 // tile of a workgroup: each XCD gets a contiguous run of tiles (it has its own L2), and runs walk 8 m tiles before the next
 // n tile, so the ~32 tiles an XCD works on at once span 8 x 4 operand panels instead of 2 x 16
 __device__ __forceinline__ void mx_tile_of(const MxDense &p, int &mt, int &nt, int &sk) {
@@ -701,11 +743,12 @@ template <typename TO, int MODE> __global__ __launch_bounds__(256, 1) void mx_de
 }
 
 // Float activations against 4-bit weights (serving: the weights are what is read).  A workgroup's four waves own 64 weight rows
-// each (or, where the layer is narrower, share the K groups) x 16 activation rows.  A K group is 512 columns: step s of it
-// takes block 4s + (lane >> 4), the row's 16 scale bytes come with one load.  Codes become bf16 with their scale applied (exact: two significant bits) and meet the activations in 16x16x32 bf16 MFMAs, whose k order is the
-// lane's block order on both operands.  The activations of a K group are converted once per workgroup and wait in LDS; fp32 ones
-// are split exactly into three bf16 terms (8 + 8 + 8 bits by truncation) and take three MFMAs: fp32 accuracy, the weights are
-// still read once.
+// each (or, where the layer is narrower, share the K groups).  A K group is 512 columns: step s of it
+// takes block 4s + (lane >> 4), the row's 16 scale bytes come with one load.  Codes become bf16 with their scale applied (exact: two significant bits) and meet
+// the activations in 16x16x32 bf16 MFMAs, whose k order is the lane's block order on both operands.  The activations of a K
+// group are converted once per workgroup and wait in LDS as columns of the product: up to 48 rows in bf16, or 16 in fp32, which
+// are split exactly into three bf16 terms (8 + 8 + 8 bits by truncation), a column each -- fp32 accuracy, and one row costs one
+// MFMA, not three.  A row's three columns are added when the waves join.
 struct Split3 { bf16 t[3]; };
 __device__ __forceinline__ Split3 split3(float x) {
   Split3 r;
@@ -720,37 +763,35 @@ __device__ __forceinline__ Split3 split3(float x) {
   return r;
 }
 constexpr int MXS_ROW = 1024 + 16;      // bytes of one activation row's K group in LDS: 512 bf16 and a pad
-template <typename TX> __global__ __launch_bounds__(256) void mx_serve_kernel(MxDense p) {
+template <typename TX, int CT> __global__ __launch_bounds__(256, 2) void mx_serve_kernel(MxDense p) {   // CT: tiles of 16 columns
   constexpr int NX = sizeof(TX) == 4 ? 3 : 1;
-  extern __shared__ __attribute__((aligned(16))) char lds[];    // [K groups of a round][NX][rows], then the partial sums
+  extern __shared__ __attribute__((aligned(1024))) char lds[];    // [K groups of a round][NX][rows], then the partial sums
   int mt, nt, sk;
   mx_small_tile(p, mt, nt, sk);
   const int lane = threadIdx.x & 63, fr = lane & 15, fq = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kw = p.kwaves, wk = wave % kw, wn = wave / kw;       // K groups taken at once; this wave's group and weight rows
-  const int m0 = mt * 16, n0 = (nt * (4 / kw) + wn) * 64;
-  const int cp = p.nb * 16, nr = max(0, min(64, p.N - n0)), rows = min(16, p.M - m0);
+  const int m0 = mt * p.xrows, n0 = (nt * (4 / kw) + wn) * 64;
+  const int cp = p.nb * 16, nr = max(0, min(64, p.N - n0)), rows = min(p.xrows, p.M - m0), cols = NX * p.xrows;
   const __amdgpu_buffer_rsrc_t wr = mx_rsrc(p.wc, nr ? n0 : 0, nr, cp), wsr = mx_rsrc(p.ws, nr ? n0 : 0, nr, p.pitch);
-  f32x4 acc[4] = {};
+  f32x4 acc[4][CT] = {};
   const int k0 = sk * p.kt_per, k1 = min(k0 + p.kt_per, (p.nb + 15) / 16);
   const int gbytes = NX * p.xrows * MXS_ROW;
   for (int kt = k0; kt < k1; kt += kw) {
-    // this wave's codes are on their way while the workgroup converts the activations
     const bool mine = kt + wk < k1;
+    const int items = min(kw, k1 - kt) * p.xrows;
+    // this wave's codes are on their way while the workgroup converts the activations
     i32x4 c[4][4], sc[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 4; ++i) {        // (rows past the operand read as zero; codes behind K meet zeros)
       const unsigned r = (unsigned)(i * 16 + fr);
       sc[i] = ld16(wsr, mine ? r * p.pitch + (kt + wk) * 16 : MX_OOB);
 #pragma unroll
-      for (int s = 0; s < 4; ++s) c[i][s] = ld16(wr, mine ? r * cp + (kt + wk) * 256 + fq * 16 + s * 64 : MX_OOB);   // (behind K: times zero)
+      for (int s = 0; s < 4; ++s) c[i][s] = ld16(wr, mine ? r * cp + (kt + wk) * 256 + fq * 16 + s * 64 : MX_OOB);
     }
-    if (kt > k0) __syncthreads();
-    // 8 columns a thread: 64 threads a row and K group
-    const int items = min(kw, k1 - kt) * p.xrows;
-    for (int t = wave; t < items; t += 4) {
-      const int col = lane * 8, g = t / p.xrows, row = t - g * p.xrows;
-      const int k = (kt + g) * 512 + col;
+    if (kt > k0) __syncthreads();        // (everyone has left the last round's activations)
+    for (int t = wave; t < items; t += 4) {      // 512 columns of a row, 8 a lane
+      const int col = lane * 8, g = t / p.xrows, row = t - g * p.xrows, k = (kt + g) * 512 + col;
       float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       if (row < rows && k < p.K) load8((const TX *)p.x + (int64_t)(m0 + row) * p.ldx + k, p.K - k, v);
       bf16x8 o[NX];
@@ -768,42 +809,47 @@ template <typename TX> __global__ __launch_bounds__(256) void mx_serve_kernel(Mx
     }
     __syncthreads();
     if (!mine) continue;      // (uniform; no weights, and zero times an infinite activation is not zero)
-    // (lanes past the rows there are read row 0: a column of the product that nobody stores)
-    const char *xl = lds + wk * gbytes + (fr < p.xrows ? fr : 0) * MXS_ROW + fq * 64;
+    const char *xl[CT];       // (lanes past the columns there are read column 0: nobody adds or stores what comes of it)
+#pragma unroll
+    for (int t = 0; t < CT; ++t) xl[t] = lds + wk * gbytes + (t * 16 + fr < cols ? t * 16 + fr : 0) * MXS_ROW + fq * 64;
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       float sf[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        sf[i] = mx_scale_or_nan(((unsigned)sc[i][s] >> (8 * fq)) & 255u);
-      }
+      for (int i = 0; i < 4; ++i) sf[i] = mx_scale_or_nan(((unsigned)sc[i][s] >> (8 * fq)) & 255u);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        bf16x8 xb[NX];
+        bf16x8 xb[CT], wv[4];
 #pragma unroll
-        for (int u = 0; u < NX; ++u) xb[u] = *(const bf16x8 *)(xl + u * p.xrows * MXS_ROW + s * 256 + j * 16);
+        for (int t = 0; t < CT; ++t) xb[t] = *(const bf16x8 *)(xl[t] + s * 256 + j * 16);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const bf16x8 wv = mx_bf16x8((unsigned)c[i][s][j], sf[i]);
+        for (int i = 0; i < 4; ++i) wv[i] = mx_bf16x8((unsigned)c[i][s][j], sf[i]);
 #pragma unroll
-          for (int u = NX - 1; u >= 0; --u) acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv, xb[u], acc[i], 0, 0, 0);
-        }
+        for (int t = 0; t < CT; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[i][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wv[i], xb[t], acc[i][t], 0, 0, 0);
       }
     }
   }
-  if (kw > 1) {          // the waves of one weight tile join
-    __syncthreads();
-    f32x4 *part = (f32x4 *)lds;
+  // join: the waves of one weight tile, and the columns of one row; each of the kw waves finishes its share of the fragments
+  __syncthreads();
+  f32x4 *const part = (f32x4 *)lds;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) part[(wave * 4 + i) * 64 + lane] = acc[i];
-    __syncthreads();
-    if (wk) return;
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      for (int w = 1; w < kw; ++w) acc[i] += part[((wave + w) * 4 + i) * 64 + lane];
-  }
+    for (int t = 0; t < CT; ++t) part[((wave * 4 + i) * CT + t) * 64 + lane] = acc[i][t];
+  __syncthreads();
+  for (int i = wk; i < 4; i += kw)
+    for (int m = fr; m < rows; m += 16) {
+      f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+      for (int w = 0; w < kw; ++w)
 #pragma unroll
-  for (int i = 0; i < 4; ++i) mx_emit(p, sk, m0 + fr, n0 + i * 16 + fq * 4, acc[i]);
+        for (int u = NX - 1; u >= 0; --u) {
+          const int col = u * p.xrows + m;
+          sum += part[(((wn * kw + w) * 4 + i) * CT + (col >> 4)) * 64 + (col & 15) + 16 * fq];
+        }
+      mx_emit(p, sk, m0 + m, n0 + i * 16 + fq * 4, sum);
+    }
 }
 
 static int mx_check(int64_t m, int64_t n, int64_t k) {
@@ -820,7 +866,7 @@ static void mx_split(MxDense &p, int groups, int64_t want) {   // K slices of wh
 }
 static int mx_serve_bytes(const MxDense &p, int x_kind) {   // LDS of the float-activation kernel
   const int groups = p.kt_per < p.kwaves ? p.kt_per : p.kwaves;
-  const int x = groups * (x_kind == CFD_MX_X_BF16 ? 1 : 3) * p.xrows * MXS_ROW, sums = p.kwaves > 1 ? 4 * 4 * 64 * 16 : 0;
+  const int cols = (x_kind == CFD_MX_X_BF16 ? 1 : 3) * p.xrows, x = groups * cols * MXS_ROW, sums = 16 * ((cols + 15) / 16) * 1024;
   return x > sums ? x : sums;
 }
 static void mx_plan(MxDense &p, int x_kind) {
@@ -839,18 +885,19 @@ static void mx_plan(MxDense &p, int x_kind) {
     const int64_t want = 256 / ((int64_t)p.nt * p.mt);
     mx_split(p, groups, want < groups / 4 ? want : groups / 4);
   } else if (serve) {
-    p.mt = (p.M + 15) / 16;
-    p.xrows = p.M < 16 ? p.M : 16;
+    const int most = x_kind == CFD_MX_X_BF16 ? 48 : 16;
+    p.mt = (p.M + most - 1) / most;
+    p.xrows = (p.M + p.mt - 1) / p.mt;
     for (p.kwaves = p.N <= 64 ? 4 : p.N <= 128 ? 2 : 1;; p.kwaves /= 2) {   // (fewer where their activations exceed the LDS)
       p.nt = (p.N + 256 / p.kwaves - 1) / (256 / p.kwaves);
       mx_split(p, (p.nb + 15) / 16, 512 / ((int64_t)p.nt * p.mt));
-      if (p.kwaves == 1 || mx_serve_bytes(p, x_kind) <= 128 * 1024) break;
+      if (p.kwaves == 1 || mx_serve_bytes(p, x_kind) <= 160 * 1024) break;
     }
   } else {
     p.nt = (p.N + 63) / 64;
     p.mt = (p.M + 63) / 64;
-    const int groups = p.pitch / 16;     // two workgroups per CU; a slice has a group for each of the four waves
-    const int64_t want = 512 / ((int64_t)p.nt * p.mt);
+    const int groups = p.pitch / 16;     // one workgroup per CU; a slice has a group for each of the four waves
+    const int64_t want = 256 / ((int64_t)p.nt * p.mt);
     mx_split(p, groups, want < groups / 4 ? want : groups / 4);
   }
 }
@@ -965,15 +1012,17 @@ extern "C" int cfd_mxfp4_dense(const cfd_mxfp4_dense_desc *d, const void *x, con
     if (int rc = set_max_lds((const void *)fn, MXT_LDS)) return rc;
     hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(256), MXT_LDS, st, p);
   } else if (!serve) {
-    hipLaunchKernelGGL(mx_dense_kernel, dim3((unsigned)blocks), dim3(256), 0, st, p);
+    if (int rc = set_max_lds((const void *)mx_dense_kernel, MXD_LDS)) return rc;
+    hipLaunchKernelGGL(mx_dense_kernel, dim3((unsigned)blocks), dim3(256), MXD_LDS, st, p);
   } else {
     const bool b16 = d->x_kind == CFD_MX_X_BF16;
     const int bytes = mx_serve_bytes(p, d->x_kind);
-    const void *fn = b16 ? (const void *)mx_serve_kernel<bf16> : (const void *)mx_serve_kernel<float>;
-    if (bytes > 64 * 1024)
-      if (int rc = set_max_lds(fn, bytes)) return rc;
-    if (b16) hipLaunchKernelGGL(mx_serve_kernel<bf16>, dim3((unsigned)blocks), dim3(256), bytes, st, p);
-    else hipLaunchKernelGGL(mx_serve_kernel<float>, dim3((unsigned)blocks), dim3(256), bytes, st, p);
+    const int tiles = ((b16 ? 1 : 3) * p.xrows + 15) / 16;
+    void (*const fns[2][3])(MxDense) = {{mx_serve_kernel<float, 1>, mx_serve_kernel<float, 2>, mx_serve_kernel<float, 3>},
+                                        {mx_serve_kernel<bf16, 1>, mx_serve_kernel<bf16, 2>, mx_serve_kernel<bf16, 3>}};
+    void (*const fn)(MxDense) = fns[b16][tiles - 1];
+    if (int rc = set_max_lds((const void *)fn, bytes)) return rc;
+    hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(256), bytes, st, p);
   }
   CFD_LAUNCH_CHECK();
   if (p.split > 1) {
