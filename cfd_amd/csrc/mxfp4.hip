@@ -896,8 +896,10 @@ static void mx_plan(MxDense &p, int x_kind) {
   } else {
     p.nt = (p.N + 63) / 64;
     p.mt = (p.M + 63) / 64;
-    const int groups = p.pitch / 16;     // one workgroup per CU; a slice has a group for each of the four waves
-    const int64_t want = 256 / ((int64_t)p.nt * p.mt);
+    // one workgroup per CU; a slice has a group for each of the four waves; no slices where half the CUs have a tile (128 x 4096 x 4096:
+    // 15.3 us in two slices, whose sum is a launch of its own, 10.2 in one)
+    const int groups = p.pitch / 16;
+    const int64_t tiles = (int64_t)p.nt * p.mt, want = tiles >= 128 ? 1 : 256 / tiles;
     mx_split(p, groups, want < groups / 4 ? want : groups / 4);
   }
 }
