@@ -356,10 +356,11 @@ int cfd_adamw_step(const cfd_adamw_tensor *tensors, int count, const cfd_adamw_d
                    float *v_scale, int *step, const float *lr_device, const float *grad_scale, void *ws, void *stream);
 
 /* ---- 4-bit microscaled matrices (OCP MX: E2M1 codes, an E8M0 power of two per 32) and the Dense layer on them (no
- * counterpart in the reference; the Dense layers are DeltaP/models/generator.py:40-46).  A matrix of `rows` x `cols` blocked along its columns is
+ * counterpart in the reference; its Dense layers are DeltaP/models/generator.py:40-46).  A matrix of `rows` x `cols`
+ * blocked along its columns is
  *   codes  uint8 [rows][16 * ceil(cols / 32)], low nibble = lower column, zero past cols;
  *   scales uint8 [rows][cfd_mxfp4_scale_pitch(cols)], value 2^(byte - 127), 255 = NaN, zero past the last block.
- * Both arrays start 16-byte aligned.  1 <= cols <= 4194304; rows may be 0.
+ * The products rely on those zeros.  Both arrays start 16-byte aligned.  1 <= cols <= 4194304; rows may be 0.
  *
  * cfd_mxfp4_quantize: x [rows][ldx >= cols] fp32 / bf16 -> codes, scales (blocks along the columns) and / or codes_t, scales_t
  * (blocks along the rows: the transposed matrix, cols rows of `rows` columns); a pair may be NULL.  Scale: floor(log2 max) - 2,
@@ -371,7 +372,8 @@ int cfd_mxfp4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t ro
                          void *stream);
 /* y [m][ldy >= n] = act(x w^T + bias), fp32 accumulation.  w: n x k in 4 bits; x: m x k in 4 bits (codes in `x`, x_scales) or
  * float (x [m][ldx >= k], x_scales NULL): then the weights are read once and the activations keep their precision --
- * the form for a few rows.  bias fp32 [n] or NULL.  ws: cfd_mxfp4_dense_workspace_bytes bytes (may be 0). */
+ * the form for a few rows.  bias fp32 [n] or NULL; ldy <= 8388608.  ws: cfd_mxfp4_dense_workspace_bytes bytes (may be 0);
+ * slices of K are summed in a fixed order: same inputs, same bits. */
 typedef enum { CFD_MX_X_F32 = 0, CFD_MX_X_BF16 = 1, CFD_MX_X_MXFP4 = 2 } cfd_mxfp4_x_kind;
 typedef struct {
   int x_kind, out_dtype, act;
