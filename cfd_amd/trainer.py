@@ -74,7 +74,8 @@ class AdamW:
 
     State, flat over all tensors (segment i at offsets[i], padded to 256 with zeros), for checkpoints and inspection:
     m, v (fp32, or float8_e4m3fn / float8_e5m2 codes with m_scale, v_scale fp32: value = code * scale[element // 256]) and
-    t, the int32 device counter of the steps taken.  step() waits for nothing and allocates nothing: it can be captured."""
+    t, the int32 device counter of the steps taken; a checkpoint is copied into them.  step()
+    waits for nothing and allocates nothing: it can be captured."""
 
     def __init__(self, params, lr=1e-3, beta_1: float = 0.9, beta_2: float = ADAM_BETA_2, epsilon: float = ADAM_EPS,
                  weight_decay=0.004, state_bits: int = 32, copies=None, seed: int = 0):
@@ -99,8 +100,8 @@ class AdamW:
             raise ValueError("AdamW: state_bits must be 8 or 32")
         if not (0.0 <= beta_1 < 1.0 and 0.0 <= beta_2 < 1.0 and epsilon >= 1e-12):
             raise ValueError("AdamW: beta must be in [0, 1) and epsilon at least 1e-12")
-        if isinstance(lr, torch.Tensor) and not (lr.device == self.device and lr.dtype == torch.float32 and lr.numel() == 1):
-            raise ValueError("AdamW: a learning-rate tensor must be one fp32 element on the parameters' device")
+        if isinstance(lr, torch.Tensor):
+            self._need_scalar(lr, "AdamW: a learning-rate tensor")
         spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in self.params + (self.copies or []) if t.numel())
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("AdamW: parameters (and copies) must not overlap")
@@ -130,7 +131,12 @@ class AdamW:
         self._ptrs = self._addresses()
 
     def _addresses(self):
-        return list(map(torch.Tensor.data_ptr, self.params + (self.copies or [])))
+        state = [self.m, self.v, self.t] + ([self.m_scale, self.v_scale] if self.state_bits == 8 else [])
+        return list(map(torch.Tensor.data_ptr, self.params + (self.copies or []) + state))
+
+    def _need_scalar(self, x: torch.Tensor, what: str) -> None:
+        if not (x.device == self.device and x.dtype == torch.float32 and x.numel() == 1):
+            raise ValueError(f"{what} must be one fp32 element on the parameters' device")
 
     def step(self, grads, grad_scale=None) -> None:
         """One update from `grads` (one dense fp32 or bf16 tensor per parameter, one dtype).  grad_scale: None, or an fp32
@@ -141,12 +147,14 @@ class AdamW:
             raise ValueError("AdamW.step: one gradient per parameter, of its length")
         ops._tensor_list(grads, "AdamW.step: gradients", None, self.device.index)
         if self._addresses() != self._ptrs:
-            raise RuntimeError("AdamW: a parameter's storage was replaced after the optimizer was built")
-        if grad_scale is not None and not (grad_scale.device == self.device and grad_scale.dtype == torch.float32 and grad_scale.numel() == 1):
-            raise ValueError("AdamW.step: grad_scale must be one fp32 element on the parameters' device")
+            raise RuntimeError("AdamW: the storage of a parameter or of the state was replaced after the optimizer was built (copy into it)")
+        if grad_scale is not None:
+            self._need_scalar(grad_scale, "AdamW.step: grad_scale")
         self._grad_column[:] = list(map(torch.Tensor.data_ptr, grads))
         self._desc.g_dtype = ops._DT[grads[0].dtype]
         on_device = isinstance(self.lr, torch.Tensor)
+        if on_device:
+            self._need_scalar(self.lr, "AdamW: a learning-rate tensor")
         self._desc.lr = 0.0 if on_device else float(self.lr)
         ops.adamw_step(self._table, self._desc, self.m, self.v, self.m_scale, self.v_scale, self.t, self.lr if on_device else None,
                        grad_scale, self._ws)

@@ -310,6 +310,23 @@ def test_refusals():
     assert int(opt.t) == 0
 
 
+@pytest.mark.parametrize("bits", [32, 8])
+def test_refuses_a_replaced_state(bits):
+    """a checkpoint is copied into the state; another tensor in its place, or a learning rate that the kernel cannot read, is refused"""
+    from cfd_amd import trainer
+    for name in ("m", "v", "t") + (("m_scale", "v_scale") if bits == 8 else ()):
+        opt = trainer.AdamW([torch.zeros(300, device="cuda")], state_bits=bits)
+        setattr(opt, name, getattr(opt, name).clone())
+        with pytest.raises(RuntimeError):
+            opt.step([torch.ones(300, device="cuda")])
+    opt = trainer.AdamW([torch.zeros(300, device="cuda")], state_bits=bits)
+    for lr in (torch.zeros(1), torch.zeros(1, dtype=torch.float64, device="cuda"), torch.zeros(2, device="cuda")):
+        opt.lr = lr
+        with pytest.raises(ValueError):
+            opt.step([torch.ones(300, device="cuda")])
+    assert int(opt.t) == 0
+
+
 def test_regressor_step_on_its_parameter_store():
     """the regressor's own forward and backward, its parameters and gradients as views of the flat buffers, clipped AdamW with an 8-bit
     state writing master and compute copy, then the trained wide layer in 4 bits beside the bf16 one"""
