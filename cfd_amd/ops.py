@@ -1034,6 +1034,19 @@ def _mx_input(x: torch.Tensor, what: str) -> int:
     return ld if rows > 1 else cols
 
 
+def _share(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """two matrices with dense rows have bytes in common (columns side by side in one buffer have none)"""
+    (pa, ra, wa), (pb, rb, wb) = ((t.data_ptr(), t.stride(0) * t.element_size() if t.shape[0] > 1 else 0, t.shape[1] * t.element_size())
+                                  for t in (a, b))
+    if pa + (a.shape[0] - 1) * ra + wa <= pb or pb + (b.shape[0] - 1) * rb + wb <= pa or not (a.numel() and b.numel()):
+        return False
+    row = ra or rb
+    if not row or (ra and rb and ra != rb):
+        return True
+    d = (pa - pb) % row
+    return d < wb or d + wa > row
+
+
 def _mx_quantize(x: torch.Tensor, rows: bool, cols: bool):
     ldx = _mx_input(x, "mxfp4_quantize: x")
     R, K = x.shape
@@ -1075,6 +1088,7 @@ def mxfp4_dequantize(q: Mxfp4, dtype: torch.dtype = torch.float32, out: Optional
 def mxfp4_from_parts(codes: torch.Tensor, scales: torch.Tensor, cols: int) -> Mxfp4:
     """an Mxfp4 matrix from packed codes uint8 (rows, 16 * blocks) and one scale byte per block, uint8 (rows, blocks): the
     scales are laid out once as the kernels read them"""
+    _need(0 < cols <= 1 << 22, "mxfp4_from_parts: columns must be in 1 .. 4194304")
     nb = (int(cols) + 31) // 32
     _dev(codes)
     _need(codes.dim() == 2 and codes.dtype == torch.uint8 and codes.shape[1] == nb * 16, f"mxfp4_from_parts: codes must be uint8 (rows, {nb * 16})")
@@ -1116,13 +1130,15 @@ def mxfp4_dense(x: Union[Mxfp4, torch.Tensor], w: Mxfp4, bias: Optional[torch.Te
     _numel(bias, n, "mxfp4_dense bias", torch.float32)
     odt = out_dtype or (out.dtype if out is not None else torch.float32 if four else x.dtype)
     _need(odt in _DT, f"mxfp4_dense: out_dtype must be fp32 or bf16, is {odt}")
+    fresh = out is None
     with _on(dev):
-        if out is None:
+        if fresh:
             out = torch.empty((m, n), dtype=odt, device=xt.device)
         _need(out.shape == (m, n) and out.dtype == odt and out.get_device() == dev,
               f"mxfp4_dense: out must be {odt} {(m, n)} on w's device, is {out.dtype} {tuple(out.shape)}")
         if m == 0 or n == 0:
             return out
+        _need(four or fresh or not _share(out, x), "mxfp4_dense: out must not overlap x")
         d = Mxfp4DenseDesc(kind, _DT[odt], act, slope, m, n, k, ldx, _mx_input(out, "mxfp4_dense: out"))
         wsb = lib.cfd_mxfp4_dense_workspace_bytes(m, n, k, kind)
         if wsb < 0:

@@ -179,6 +179,38 @@ def test_dense_nan_blocks_reach_their_row_or_column_only():
         assert torch.equal(bad, want)
 
 
+@pytest.mark.parametrize("m,n,k", [(20, 70, 608), (1750, 1720, 96)])
+def test_dense_scales_at_the_ends_of_their_range(m, n, k):
+    """2^127 on one operand and 2^-127 on the other: the product is of order one, whichever side's values are subnormal"""
+    from cfd_amd import ops
+    r = np.random.default_rng(7)
+    cx, cw = r.integers(0, 16, (m, k), dtype=np.uint8), r.integers(0, 16, (n, k), dtype=np.uint8)
+    for bx, bw in ((254, 0), (0, 254), (127, 127)):
+        sx, sw = np.full((m, (k + 31) // 32), bx, np.uint8), np.full((n, (k + 31) // 32), bw, np.uint8)
+        xq, wq = (ops.mxfp4_from_parts(torch.from_numpy(O.pack(c)).cuda(), torch.from_numpy(s).cuda(), k) for c, s in ((cx, sx), (cw, sw)))
+        _close(ops.mxfp4_dense(xq, wq), O.values(cx, sx, k), O.values(cw, sw, k), None, 0)
+    sw = np.zeros((n, (k + 31) // 32), np.uint8)
+    wq = ops.mxfp4_from_parts(torch.from_numpy(O.pack(cw)).cuda(), torch.from_numpy(sw).cuda(), k)
+    x = (torch.randn(20, k, generator=torch.Generator().manual_seed(8)) * 2.0 ** 124).cuda()
+    for t in (x, x.bfloat16()):
+        _close(ops.mxfp4_dense(t, wq, out_dtype=torch.float32), _np(t), O.values(cw, sw, k), None, 0)
+
+
+def test_dense_output_beside_its_activations():
+    """columns of one buffer: the output's next to the activations' is a concat in place, over them is refused"""
+    from cfd_amd import _lib, ops
+    w = ops.mxfp4_quantize(_rnd(24, 40, 71, spread=0.0).cuda())
+    buf = torch.zeros(6, 64, device="cuda")
+    buf[:, :40] = _rnd(6, 40, 72, spread=0.0).cuda()
+    want = ops.mxfp4_dense(buf[:, :40].contiguous(), w)
+    kept = buf[:, :40].clone()
+    ops.mxfp4_dense(buf[:, :40], w, out=buf[:, 40:])
+    assert torch.equal(buf[:, 40:], want) and torch.equal(buf[:, :40], kept)
+    for out in (buf[:, 39:63], buf[:, :24], buf.view(-1)[:144].view(6, 24)):
+        with pytest.raises(_lib.CfdError):
+            ops.mxfp4_dense(buf[:, :40], w, out=out)
+
+
 def test_empty():
     from cfd_amd import ops
     w = ops.mxfp4_quantize(torch.ones(4, 40, device="cuda"))
@@ -321,3 +353,6 @@ def test_refusals():
         ops.mxfp4_dequantize(q, torch.float16)
     with bad:
         ops.mxfp4_from_parts(q.codes, q.scales, 40)
+    for cols in (0, -5, 1 << 23):
+        with bad:
+            ops.mxfp4_from_parts(q.codes, q.scales[:, :2], cols)
