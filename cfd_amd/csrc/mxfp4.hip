@@ -60,7 +60,7 @@ __device__ __forceinline__ unsigned mx_scale_byte(unsigned amax) {
 }
 // the hardware conversions take the scale as an fp32 power of two; a byte of 0 is the subnormal 2^-127
 __device__ __forceinline__ float mx_scale_f32(unsigned byte) {
-  return __uint_as_float(byte ? byte << 23 : 0x00400000u);
+  return __uint_as_float(max(byte << 23, 0x00400000u));
 }
 __device__ __forceinline__ unsigned mx_code8(const float (&x)[8], unsigned byte) {
   const float s = mx_scale_f32(byte);
@@ -204,8 +204,27 @@ template <typename T> __global__ __launch_bounds__(256) void mx_quant_both_kerne
     Eight<T> v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i].load(src0 + i * 16 * ldx);
+    const int sw = tid >> 4;
+    if (codes) {       // (no element is past an end: half the instructions of `put`: 4096 x 4096 bf16 15.2 -> 14.2 us)
+      uint8_t *const to = codes + (int64_t)(r0 + sw) * nb * 16 + (c0 + c) / 2;
+      unsigned bytes[2] = {0, 0};
 #pragma unroll
-    for (int i = 0; i < 8; ++i) put(i, v[i]);
+      for (int i = 0; i < 8; ++i) {
+        v[i].to_lds(tile + (i * 16 + sw) * W + ((c * (int)sizeof(T) / 4) ^ ((i >> 1) * 16)));
+        const unsigned byte = mx_scale_byte(quad_umax(amax8(v[i].get())));
+        *(unsigned *)(to + (int64_t)i * nb * 256) = mx_code8(v[i].get(), byte);
+        bytes[i >> 2] |= byte << (8 * (i & 3));
+      }
+      // the four lanes of a block hold its byte of eight rows: each stores two of them
+      uint8_t *const sc = scales + (int64_t)(r0 + (tid & 3) * 16 + sw) * pitch + ((c0 + c) >> 5);
+      sc[0] = (uint8_t)(bytes[0] >> (8 * (tid & 3)));
+      sc[(int64_t)64 * pitch] = (uint8_t)(bytes[1] >> (8 * (tid & 3)));
+      if (c0 + QT == K)      // the zeros behind the last block
+        for (int i = nb + (tid & 1) * 4; i < pitch; i += 8) *(unsigned *)(scales + (int64_t)(r0 + (tid >> 1)) * pitch + i) = 0u;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i].to_lds(tile + (i * 16 + sw) * W + ((c * (int)sizeof(T) / 4) ^ ((i >> 1) * 16)));
+    }
   } else {
     for (int i = 0; i < 8; ++i) {
       Eight<T> v;

@@ -50,6 +50,18 @@ def test_quantize(shape, dtype):
     _same(ops.mxfp4_quantize(wide[:, 3:3 + shape[1]]), x)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("shape", [(128, 128), (128, 640), (400, 384), (256, 512), (640, 128)])
+def test_quantize_both_in_whole_tiles(shape, dtype):
+    """matrices that end with a 128-column tile: scales behind the last block are zero, a NaN stays in its two blocks"""
+    from cfd_amd import ops
+    x = _rnd(*shape, 2, dtype).cuda()
+    x[127, 127] = float("nan")
+    q, t = ops.mxfp4_quantize_both(x)
+    _same(q, x)
+    _same(t, x.t())
+
+
 def test_quantize_special_blocks():
     from cfd_amd import ops
     rows = []
