@@ -223,6 +223,35 @@ def test_dense_output_beside_its_activations():
             ops.mxfp4_dense(buf[:, :40], w, out=out)
 
 
+@pytest.mark.parametrize("m,n,k", [(65, 63, 257), (3, 129, 600), (1999, 1537, 515), (260, 250, 65536), (2048, 1536, 512)])
+def test_nothing_behind_the_last_row_is_written(m, n, k):
+    from cfd_amd import _lib, ops
+    lib, st = _lib.load(), torch.cuda.current_stream().cuda_stream
+    x, w = _rnd(m, k, 81, spread=0.5).cuda(), ops.mxfp4_quantize(_rnd(n, k, 82, spread=0.5).cuda())
+    xq = ops.mxfp4_quantize(x)
+    for dtype in (torch.float32, torch.bfloat16):
+        for a in (xq, x[:40]):
+            rows = a.shape[0]
+            buf = torch.full((rows + 3, n + n % 2), 5.0, dtype=dtype, device="cuda")
+            ops.mxfp4_dense(a, w, out=buf[:rows, :n])
+            assert torch.equal(buf[:rows, :n], ops.mxfp4_dense(a, w, out_dtype=dtype))
+            assert (buf[rows:] == 5).all() and (buf[:, n:] == 5).all()
+        buf = torch.full((m + 2, k), 5.0, dtype=dtype, device="cuda")
+        ops.mxfp4_dequantize(xq, out=buf[:m])
+        assert (buf[m:] == 5).all()
+        xd = x.to(dtype)
+        q, t = ops.mxfp4_quantize_both(xd)
+        ends = []
+        for part in (q.codes, q.scales, t.codes, t.scales):       # each array with 4 KiB behind it
+            ends.append(torch.full((part.numel() + 4096,), 77, dtype=torch.uint8, device="cuda"))
+        for ptrs in ([e.data_ptr() for e in ends], [ends[0].data_ptr(), ends[1].data_ptr(), None, None], [None, None, ends[2].data_ptr(), ends[3].data_ptr()]):
+            _lib.check(lib.cfd_mxfp4_quantize(xd.data_ptr(), k, ops._DT[dtype], m, k, *ptrs, st), "cfd_mxfp4_quantize")
+            for e, part, p in zip(ends, (q.codes, q.scales, t.codes, t.scales), ptrs):
+                if p is not None:
+                    assert torch.equal(e[:part.numel()], part.view(-1))
+                assert (e[part.numel():] == 77).all()
+
+
 def test_empty():
     from cfd_amd import ops
     w = ops.mxfp4_quantize(torch.ones(4, 40, device="cuda"))
