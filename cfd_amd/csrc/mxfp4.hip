@@ -173,8 +173,8 @@ template <typename T> __global__ __launch_bounds__(256) void mx_quant_rows_kerne
 
 // both orientations from one read: a 128 x 128 tile; rows are coded on the way in, columns from LDS, two adjacent columns and 32
 // rows a thread.  LDS words are swizzled by 16 per 32 rows: the four row blocks that a quad of lanes reads lie in different banks.
-// Codes leave as 64 contiguous bytes a row in both orientations, scales as 32-bit words: these short runs and the turn in LDS hold it
-// under a copy's rate (4090 x 4102 fp32, 85 MB: 22.5 us, 3.8 TB/s).
+// Codes leave as 64 contiguous bytes a row in both orientations.  Near a copy's rate where there are tiles for several rounds (8192 x 4096
+// fp32, 170 MB: 35 us, 4.9 TB/s); one round fills and drains the chip in ~4 us beside the bytes' time (4090 x 4102, 85 MB: 22.2 us).
 constexpr int QT = 128;
 template <typename T> __global__ __launch_bounds__(256) void mx_quant_both_kernel(const T *x, int64_t ldx, int R, int K,
                                                                                    int nb, int pitch, uint8_t *codes,
