@@ -542,11 +542,13 @@ __device__ __forceinline__ f32x16 mx_mma(int s, i32x4 a, i32x4 b, f32x16 c, int 
     default: return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wide(a), wide(b), c, 4, 4, 3, as, 3, bs);
   }
 }
-// tile of a workgroup: each XCD gets a contiguous run of tiles (it has its own L2), and runs walk 8 m tiles before the next
-// n tile, so the ~32 tiles an XCD works on at once span 8 x 4 operand panels instead of 2 x 16
+// tile of a workgroup: of the 256 that run at once each XCD (it has its own L2) gets 32 that follow each other, 8 m tiles before the next n
+// tile: 8 x 4 operand panels instead of 2 x 16.  The XCDs' runs are neighbours, so what is written at a time spreads over the
+// whole width of the output (one long run for each XCD sets them a power of two apart and they meet in the same memory channels:
+// 8192^2 x 512 to bf16 50 -> 43 us, to fp32 80 -> 72; 8192^3 to fp32 263 -> 254; 16384 x 4096^2 to fp32 151 -> 155)
 __device__ __forceinline__ void mx_tile_of(const MxDense &p, int &mt, int &nt, int &sk) {
-  const int nwg = p.mt * p.nt * p.split, q = nwg >> 3, r = nwg & 7, xcd = blockIdx.x & 7;
-  int t = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + ((int)blockIdx.x >> 3);
+  const int first = (int)blockIdx.x & ~255, some = min(256, p.mt * p.nt * p.split - first), q = some >> 3, r = some & 7, xcd = blockIdx.x & 7;
+  int t = first + (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (((int)blockIdx.x & 255) >> 3);
   sk = t / (p.mt * p.nt);
   t -= sk * p.mt * p.nt;
   const int g = t / (8 * p.nt), h = min(8, p.mt - g * 8), u = t - g * 8 * p.nt;
