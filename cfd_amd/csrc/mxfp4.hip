@@ -767,7 +767,7 @@ template <typename TO, int MODE> __global__ __launch_bounds__(256, 1) void mx_de
 }
 
 // Float activations against 4-bit weights (serving: the weights are what is read).  A workgroup's four waves own 64 weight rows
-// each (or, where the layer is narrower, share the K groups).  A K group is 512 columns: step s of it
+// each, or share the K groups of 64 rows (`mx_plan` chooses).  A K group is 512 columns: step s of it
 // takes block 4s + (lane >> 4), the row's 16 scale bytes come with one load.  Codes become bf16 with their scale applied (exact: two significant bits) and meet
 // the activations in 16x16x32 bf16 MFMAs, whose k order is the lane's block order on both operands.  The activations of a K
 // group are converted once per workgroup and wait in LDS as columns of the product: up to 48 rows in bf16, or 16 in fp32, which
@@ -913,9 +913,16 @@ static void mx_plan(MxDense &p, int x_kind) {
     const int most = x_kind == CFD_MX_X_BF16 ? 48 : 16;
     p.mt = (p.M + most - 1) / most;
     p.xrows = (p.M + p.mt - 1) / p.mt;
-    for (p.kwaves = p.N <= 64 ? 4 : p.N <= 128 ? 2 : 1;; p.kwaves /= 2) {   // (fewer where their activations exceed the LDS)
+    // Four waves on one weight tile where each has one K group, or its few columns are cheap to convert four times as often: a
+    // wave's loads of 16 rows at a time keep a CU's address unit busy, and so they spread over more CUs.  Us, four waves on a tile | four
+    // tiles: 1 row fp32 256 x 2048 7.1 | 9.0, 256 x 262144 14.0 | 16.9, 28672 x 8192 27.2 | 36.0; 16 rows bf16 4096^2 11.1 | 12.3, 8192^2
+    // 19.8 | 19.3, 28672 x 8192 50 | 42; 48 rows bf16 256 x 2048 13.0 | 17.8, 256 x 65536 18.9 | 21.7, 1030 x 16384 31 | 20
+    const int groups = (p.nb + 15) / 16, cols = (x_kind == CFD_MX_X_BF16 ? 1 : 3) * p.xrows;
+    const int64_t units = (int64_t)((p.N + 63) / 64) * p.mt * groups;
+    const bool spread = units <= 512 || (cols <= 16 && units * cols <= 32768);
+    for (p.kwaves = spread || p.N <= 64 ? 4 : p.N <= 128 ? 2 : 1;; p.kwaves /= 2) {   // (fewer where their activations exceed the LDS)
       p.nt = (p.N + 256 / p.kwaves - 1) / (256 / p.kwaves);
-      mx_split(p, (p.nb + 15) / 16, 512 / ((int64_t)p.nt * p.mt));
+      mx_split(p, groups, 512 / ((int64_t)p.nt * p.mt));
       if (p.kwaves == 1 || mx_serve_bytes(p, x_kind) <= 160 * 1024) break;
     }
   } else {

@@ -164,6 +164,18 @@ def test_dense_float_activations(m, n, k, dtype):
     assert torch.equal(ops.mxfp4_dense(wide[:, 1:1 + k], wq, out_dtype=torch.float32), y)
 
 
+@pytest.mark.parametrize("m,n,k,dtype", [(48, 60, 300000, torch.bfloat16), (16, 100, 140000, torch.float32), (16, 1030, 17000, torch.float32),
+                                         (1, 1030, 17000, torch.float32), (1, 40000, 9000, torch.float32), (49, 200, 5000, torch.bfloat16)])
+def test_dense_float_activations_shared_between_waves(m, n, k, dtype):
+    """one, two and four waves on a weight tile, one and several K groups each, and rows in more than one tile"""
+    from cfd_amd import ops
+    x, w = _rnd(m, k, 91, dtype, 0.5).cuda(), ops.mxfp4_quantize(_rnd(n, k, 92, spread=0.5).cuda())
+    w64 = _np(ops.mxfp4_dequantize(w))
+    y = ops.mxfp4_dense(x, w, out_dtype=torch.float32)
+    _close(y, _np(x), w64, None, 0)
+    assert torch.equal(y, ops.mxfp4_dense(x, w, out_dtype=torch.float32))
+
+
 def test_dense_float_activations_at_the_ends_of_the_range():
     """activations that a bf16 rounding would push to infinity, infinities and NaN: only the rows that hold them change"""
     from cfd_amd import ops
