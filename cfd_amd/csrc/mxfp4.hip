@@ -920,9 +920,12 @@ static void mx_plan(MxDense &p, int x_kind) {
     const int groups = (p.nb + 15) / 16, cols = (x_kind == CFD_MX_X_BF16 ? 1 : 3) * p.xrows;
     const int64_t units = (int64_t)((p.N + 63) / 64) * p.mt * groups;
     const bool spread = units <= 512 || (cols <= 16 && units * cols <= 32768);
+    // ... and no slices, whose sum is a launch of its own, where the four waves have all the groups at few columns: one fp32 row 4096 x 1024
+    // 6.2 | 7.3, 1030 x 2048 6.9 | 7.4 us, and 2.7 us less of the host's time; eight bf16 rows 8192 x 1024 6.5 | 7.5, but 1030 x 2048 8.4 | 7.1
+    const bool whole = spread && groups <= 4 && cols <= (groups <= 2 ? 16 : 6);
     for (p.kwaves = spread || p.N <= 64 ? 4 : p.N <= 128 ? 2 : 1;; p.kwaves /= 2) {   // (fewer where their activations exceed the LDS)
       p.nt = (p.N + 256 / p.kwaves - 1) / (256 / p.kwaves);
-      mx_split(p, groups, 512 / ((int64_t)p.nt * p.mt));
+      mx_split(p, groups, whole ? 1 : 512 / ((int64_t)p.nt * p.mt));
       if (p.kwaves == 1 || mx_serve_bytes(p, x_kind) <= 160 * 1024) break;
     }
   } else {

@@ -165,7 +165,8 @@ def test_dense_float_activations(m, n, k, dtype):
 
 
 @pytest.mark.parametrize("m,n,k,dtype", [(48, 60, 300000, torch.bfloat16), (16, 100, 140000, torch.float32), (16, 1030, 17000, torch.float32),
-                                         (1, 1030, 17000, torch.float32), (1, 40000, 9000, torch.float32), (49, 200, 5000, torch.bfloat16)])
+                                         (1, 1030, 17000, torch.float32), (1, 40000, 9000, torch.float32), (49, 200, 5000, torch.bfloat16),
+                                         (2, 1030, 2040, torch.float32), (5, 300, 1000, torch.float32), (16, 70, 900, torch.bfloat16), (6, 70, 1900, torch.bfloat16)])
 def test_dense_float_activations_shared_between_waves(m, n, k, dtype):
     """one, two and four waves on a weight tile, one and several K groups each, and rows in more than one tile"""
     from cfd_amd import ops
