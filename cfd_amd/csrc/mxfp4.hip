@@ -772,8 +772,8 @@ template <typename TO, int MODE> __global__ __launch_bounds__(256, 1) void mx_de
 // the activations in 16x16x32 bf16 MFMAs, whose k order is the lane's block order on both operands.  The activations of a K
 // group are converted once per workgroup and wait in LDS as columns of the product: up to 48 rows in bf16, or 16 in fp32, which
 // are split exactly into three bf16 terms (8 + 8 + 8 bits by truncation), a column each -- fp32 accuracy, and one row costs one
-// MFMA, not three.  A row's three columns are added when the waves join.  One fp32 row on 262144 x 256 (36 MB): 12.1 us, the latency of one round
-// of loads on top of 3.0 TB/s; the slices' sum takes 3.8 more.
+// MFMA, not three.  A row's three columns are added when the waves join.  One fp32 row on 262144 x 256 (36 MB): 10.8 us, the latency of one round
+// of loads on top of 3.3 TB/s; the slices' sum takes 3.8 more.
 struct Split3 { bf16 t[3]; };
 __device__ __forceinline__ Split3 split3(float x) {
   Split3 r;
