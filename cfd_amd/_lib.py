@@ -107,6 +107,7 @@ SIGNATURES = {
     "cfd_mxfp4_quantize": (_i, [_vp, _i64, _i, _i64, _i64, _vp, _vp, _vp, _vp, _vp]),
     "cfd_mxfp4_dequantize": (_i, [_vp, _vp, _i64, _i64, _vp, _i64, _i, _vp]),
     "cfd_mxfp4_dense_workspace_bytes": (_i64, [_i64, _i64, _i64, _i]),
+    "cfd_mxfp4_dense_plan": (_i, [_i64, _i64, _i64, _i, C.POINTER(C.c_int)]),
     "cfd_mxfp4_dense": (_i, [C.POINTER(Mxfp4DenseDesc), _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "cfd_bn_update_moving": (_i, [_vp, _vp, _vp, _vp, _i, _i, _f, _vp]),
     "cfd_bn_update_moving_multi": (_i, [_i, _vp, _vp, _vp, _vp, _vp, _i, _f, _vp]),

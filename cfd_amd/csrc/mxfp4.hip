@@ -1015,6 +1015,21 @@ extern "C" int64_t cfd_mxfp4_dense_workspace_bytes(int64_t m, int64_t n, int64_t
   return p.split > 1 ? (int64_t)p.split * m * n * 4 : 0;
 }
 
+extern "C" int cfd_mxfp4_dense_plan(int64_t m, int64_t n, int64_t k, int x_kind, int *plan) {
+  if (int rc = mx_check(m, n, k)) return rc;
+  CFD_REQUIRE(x_kind >= CFD_MX_X_F32 && x_kind <= CFD_MX_X_MXFP4, "bad x_kind");
+  CFD_REQUIRE(plan && m && n, "bad arguments");
+  MxDense p = {};
+  p.M = (int)m; p.N = (int)n; p.K = (int)k;
+  mx_plan(p, x_kind);
+  const bool serve = x_kind != CFD_MX_X_MXFP4;
+  plan[0] = p.big ? 256 : serve ? p.xrows : 64;
+  plan[1] = p.split;
+  plan[2] = p.kt_per;
+  plan[3] = p.big ? 1 : serve ? p.kwaves : 4;
+  return CFD_OK;
+}
+
 extern "C" int cfd_mxfp4_dense(const cfd_mxfp4_dense_desc *d, const void *x, const uint8_t *x_scales, const uint8_t *w_codes,
                                const uint8_t *w_scales, const float *bias, void *y, void *ws, void *stream) {
   CFD_REQUIRE(d, "NULL descriptor");

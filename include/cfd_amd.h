@@ -381,6 +381,9 @@ typedef struct {
   int64_t m, n, k, ldx, ldy;
 } cfd_mxfp4_dense_desc;
 int64_t cfd_mxfp4_dense_workspace_bytes(int64_t m, int64_t n, int64_t k, int x_kind);
+/* how that product is divided, for tests and tuning (m, n > 0; launches nothing): plan[0] = output rows of a tile, plan[1] = slices
+ * of K, plan[2] = K groups of 512 columns in a slice, plan[3] = waves that take a tile's groups in turn */
+int cfd_mxfp4_dense_plan(int64_t m, int64_t n, int64_t k, int x_kind, int *plan);
 int cfd_mxfp4_dense(const cfd_mxfp4_dense_desc *desc, const void *x, const uint8_t *x_scales, const uint8_t *w_codes,
                     const uint8_t *w_scales, const float *bias, void *y, void *ws, void *stream);
 

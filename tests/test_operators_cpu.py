@@ -132,3 +132,24 @@ def test_oracle_adamw_published_first_step():
     p, m, v = OO.adamw(10.0, 3.0, 0.0, 0.0, 1, 0.1, 0.9, 0.999, 1e-7, 0.0)
     assert abs(p - 9.9) < 1e-6 and math.isclose(float(m), 0.3) and math.isclose(float(v), 0.009)
     assert OO.grad_norm([[3.0], [4.0]], 1.0) == (5.0, 0.2)
+
+
+def test_mxfp4_plan_reaches_every_way_of_sharing(lib):
+    """the products that the GPU tests compute exactly are divided as their lists say: one, two and four waves on a weight tile, with
+    one round over the K groups and several, whole and ragged, in one slice of K and in many; both 4-bit tiles with and without slices"""
+    from tests import test_mxfp4_sums_gpu as T
+    seen = set()
+    for m, n, k, kind, how in T.FLOAT:
+        rows, slices, groups, waves = T.plan(lib, m, n, k, kind)
+        total = -(-k // 512)
+        last = total - (slices - 1) * groups
+        assert (waves, -(-groups // waves), bool(groups % waves or last % waves), slices) == how, (m, n, k, kind)
+        seen |= {(waves, "rounds", groups > waves), (waves, "ragged", how[2]), (waves, "slices", slices > 1), (kind, waves)}
+    assert {(w, "rounds", True) for w in (1, 2, 4)} | {(w, "rounds", False) for w in (2, 4)} <= seen
+    assert {(w, "ragged", r) for w in (2, 4) for r in (True, False)} <= seen
+    assert {(t, w) for t in ("fp32", "bf16") for w in (1, 2, 4)} | {(4, "slices", False), (4, "slices", True)} <= seen
+    four = [T.plan(lib, m, n, k, "fp4") for m, n, k, _ in T.FOUR]
+    assert [(rows, groups, slices) for rows, slices, groups, _ in four] == [how for *_, how in T.FOUR]
+    assert {(rows, slices > 1) for rows, slices, *_ in four} == {(r, s) for r in (64, 256) for s in (True, False)}
+    assert lib.cfd_mxfp4_dense_plan(4, 4, 0, 2, None) < 0 and lib.cfd_mxfp4_dense_plan(4, 4, 64, 3, (C.c_int * 4)()) < 0
+    _refused(lib, lib.cfd_mxfp4_dense_plan(0, 4, 64, 2, (C.c_int * 4)()), "bad arguments")
