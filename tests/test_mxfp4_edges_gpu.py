@@ -1,0 +1,34 @@
+"""4-bit matrices and the Dense layer on them where values, views and types meet their ends."""
+import pytest
+import torch
+
+from tests.test_mxfp4_gpu import O, _np, _same
+
+pytestmark = pytest.mark.gpu
+
+
+def test_quantize_special_blocks_bf16():
+    """ties and borders at several scales, subnormals, zeros, infinities and NaN: bf16 blocks are examined as they lie in memory,
+    on ragged tiles and on whole ones"""
+    from cfd_amd import ops
+    rows = []
+    top = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0, 6.96875, 0.2490234375, 0.251953125, 4.96875, 5.03125, -5.0, -0.0])
+    for e in (-126, -40, 0, 3, 100, 124):
+        for biggest in (4.0, 6.0, 7.0, 7.03125):                # (7.03125: the next one over 7)
+            rows.append(torch.cat([top.clamp(-biggest, biggest), torch.full((15,), 0.30078125), torch.tensor([biggest])]) * 2.0 ** e)
+    rows += [torch.zeros(32), torch.full((32,), -0.0), torch.full((32,), 2.0 ** -133), torch.linspace(-1.1e-38, 1.1e-38, 32),
+             torch.full((32,), 3.3895313892515355e38)]
+    for bad in (float("inf"), -float("inf"), float("nan")):
+        rows.append(torch.arange(32.0))
+        rows[-1][7] = bad
+    x = torch.stack(rows).to(torch.bfloat16).cuda()
+    assert int((x[26] != 0).sum()) == 32                        # (2^-133 is bf16's smallest subnormal)
+    tile = torch.cat([x.roll(5 * i, 0) for i in range(4)], 1).repeat(8, 1)[:256]      # 256 x 128: two whole tiles
+    for a in (x, tile, tile[:129], torch.cat([tile, tile[:, :40]], 1)):
+        q, t = ops.mxfp4_quantize_both(a)
+        _same(q, a), _same(t, a.t())
+        _same(ops.mxfp4_quantize(a), a)
+        _same(ops.mxfp4_quantize(a, transpose=True), a.t())
+        _same(ops.mxfp4_quantize(a.t().contiguous(), transpose=True), a)
+    v = torch.from_numpy(O.round_trip(_np(x))).to(torch.bfloat16)
+    assert torch.equal(torch.nan_to_num(ops.mxfp4_dequantize(ops.mxfp4_quantize(x), torch.bfloat16).cpu()), torch.nan_to_num(v))
