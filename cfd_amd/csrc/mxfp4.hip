@@ -327,6 +327,11 @@ struct MxDense {
   bool pairs;                         //   bf16 output: two columns are one aligned word
 };
 
+// activation of a sum.  ReLU by comparison, not by a slope of zero: a sum of -infinity is 0 (its product with zero would be NaN), and NaN stays
+__device__ __forceinline__ float mx_relu(float v) { return v < 0.f ? 0.f : v; }
+__device__ __forceinline__ float mx_act(const MxDense &p, float v) {
+  return p.act == CFD_ACT_RELU ? mx_relu(v) : apply_act(v, p.act, p.slope);
+}
 __device__ __forceinline__ void mx_store(const MxDense &p, int64_t m, int n, float v) {   // one element of the output
   if (p.out_bf16) ((bf16 *)p.y)[m * p.ldy + n] = (bf16)v;
   else ((float *)p.y)[m * p.ldy + n] = v;
@@ -343,7 +348,7 @@ __device__ __forceinline__ void mx_emit(const MxDense &p, int sk, int64_t m, int
   }
 #pragma unroll
   for (int r = 0; r < 4; ++r)
-    if (n + r < p.N) mx_store(p, m, n + r, apply_act(v[r] + (p.bias ? p.bias[n + r] : 0.f), p.act, p.slope));
+    if (n + r < p.N) mx_store(p, m, n + r, mx_act(p, v[r] + (p.bias ? p.bias[n + r] : 0.f)));
 }
 
 // sums of the split slabs, bias, activation, output type: 16 lanes take 64 consecutive outputs, 16 groups of lanes take the
@@ -373,7 +378,7 @@ __global__ __launch_bounds__(256) void mx_split_sum_kernel(MxDense p) {
   for (int k = 0; k < 16; ++k) v += part[k][threadIdx.x >> 2][threadIdx.x & 3];
   const int64_t m = o / p.N;
   const int n = (int)(o - m * p.N);
-  mx_store(p, m, n, apply_act(v + (p.bias ? p.bias[n] : 0.f), p.act, p.slope));
+  mx_store(p, m, n, mx_act(p, v + (p.bias ? p.bias[n] : 0.f)));
 }
 
 constexpr unsigned MX_OOB = 0x80000000u;
@@ -558,7 +563,7 @@ __device__ __forceinline__ void mx_tile_of(const MxDense &p, int &mt, int &nt, i
   sk = __builtin_amdgcn_readfirstlane(sk);
 }
 
-enum { MX_PLAIN = 0, MX_LINEAR = 1, MX_SIGMOID = 2 };   // epilogue: the sums; bias and piecewise linear activation; bias and sigmoid
+enum { MX_PLAIN = 0, MX_LINEAR = 1, MX_RELU = 2, MX_SIGMOID = 3 };   // epilogue: the sums; bias and none or LeakyReLU; bias and ReLU; bias and sigmoid
 template <typename TO, int MODE> __global__ __launch_bounds__(256, 1) void mx_dense256_kernel(MxDense p) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int tid = threadIdx.x, lane = tid & 63;
@@ -718,6 +723,7 @@ template <typename TO, int MODE> __global__ __launch_bounds__(256, 1) void mx_de
   auto fin = [&](float v, float bv) {
     if constexpr (MODE == MX_PLAIN) return v;
     else if constexpr (MODE == MX_LINEAR) return apply_act_linear(v + bv, ns);
+    else if constexpr (MODE == MX_RELU) return mx_relu(v + bv);
     else return 1.f / (1.f + __expf(-(v + bv)));
   };
   auto put = [&](auto pairs) {
@@ -1057,9 +1063,11 @@ extern "C" int cfd_mxfp4_dense(const cfd_mxfp4_dense_desc *d, const void *x, con
   hipStream_t st = (hipStream_t)stream;
   if (p.big) {
     const bool b16 = p.out_bf16 && p.split == 1;
-    const int mode = p.split > 1 || (!bias && p.act == CFD_ACT_NONE) ? MX_PLAIN : p.act == CFD_ACT_SIGMOID ? MX_SIGMOID : MX_LINEAR;
-    void (*const fns[2][3])(MxDense) = {{mx_dense256_kernel<float, MX_PLAIN>, mx_dense256_kernel<float, MX_LINEAR>, mx_dense256_kernel<float, MX_SIGMOID>},
-                                        {mx_dense256_kernel<bf16, MX_PLAIN>, mx_dense256_kernel<bf16, MX_LINEAR>, mx_dense256_kernel<bf16, MX_SIGMOID>}};
+    const int mode = p.split > 1 || (!bias && p.act == CFD_ACT_NONE) ? MX_PLAIN : p.act == CFD_ACT_SIGMOID ? MX_SIGMOID : p.act == CFD_ACT_RELU ? MX_RELU : MX_LINEAR;
+    void (*const fns[2][4])(MxDense) = {{mx_dense256_kernel<float, MX_PLAIN>, mx_dense256_kernel<float, MX_LINEAR>, mx_dense256_kernel<float, MX_RELU>,
+                                         mx_dense256_kernel<float, MX_SIGMOID>},
+                                        {mx_dense256_kernel<bf16, MX_PLAIN>, mx_dense256_kernel<bf16, MX_LINEAR>, mx_dense256_kernel<bf16, MX_RELU>,
+                                         mx_dense256_kernel<bf16, MX_SIGMOID>}};
     void (*const fn)(MxDense) = fns[b16][mode];
     if (int rc = set_max_lds((const void *)fn, MXT_LDS)) return rc;
     hipLaunchKernelGGL(fn, dim3((unsigned)blocks), dim3(256), MXT_LDS, st, p);

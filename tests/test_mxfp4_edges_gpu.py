@@ -32,3 +32,31 @@ def test_quantize_special_blocks_bf16():
         _same(ops.mxfp4_quantize(a.t().contiguous(), transpose=True), a)
     v = torch.from_numpy(O.round_trip(_np(x))).to(torch.bfloat16)
     assert torch.equal(torch.nan_to_num(ops.mxfp4_dequantize(ops.mxfp4_quantize(x), torch.bfloat16).cpu()), torch.nan_to_num(v))
+
+
+@pytest.mark.parametrize("m,n,k,x_four", [(5, 20, 64, False), (2, 30, 40000, False), (20, 30, 64, True), (8, 8, 40000, True),
+                                          (1800, 1700, 96, True), (260, 250, 65536, True)])
+def test_activations_of_infinite_sums(m, n, k, x_four):
+    """ReLU of a sum of -infinity is 0, of NaN is NaN, in every epilogue: tiles of 16, 64 and 256 rows, with and without slices of K"""
+    from cfd_amd import ops
+    x, w = torch.zeros(m, k, device="cuda"), torch.zeros(n, k, device="cuda")
+    if x_four:                 # products of 2^254
+        x[:, 3] = 2.0 ** 127 * torch.tensor([1.0, -1.0], device="cuda").repeat(m)[:m]
+        x[m - 1, 3] = float("nan")
+        w[:, 3] = 2.0 ** 127 * torch.tensor([1.0, -1.0, 0.0], device="cuda").repeat(n)[:n]
+    else:
+        x[:, 3] = torch.tensor([float("inf"), -float("inf"), 1.0, float("nan")], device="cuda").repeat(m)[:m]
+        w[:, 3] = torch.tensor([1.0, -1.0, 0.0], device="cuda").repeat(n)[:n]
+    z = x[:, 3, None] * w[None, :, 3]
+    assert torch.isinf(z).any() and (z == -float("inf")).any()
+    a, b = ops.mxfp4_quantize(x) if x_four else x, ops.mxfp4_quantize(w)
+    bias = torch.ones(n, device="cuda")
+    for out_dtype in (torch.float32, torch.bfloat16):
+        for act, want in ((ops.ACT_RELU, torch.relu(z + 1)), (ops.ACT_LEAKY, torch.nn.functional.leaky_relu(z + 1, 0.2)),
+                          (ops.ACT_NONE, z + 1), (ops.ACT_SIGMOID, torch.sigmoid(z + 1))):
+            y = ops.mxfp4_dense(a, b, bias=bias, act=act, out_dtype=out_dtype).float()
+            tol = 2.0 ** -8 if out_dtype == torch.bfloat16 else 2.0 ** -20
+            same = (y == want) | (torch.isnan(y) & torch.isnan(want)) | ((y - want).abs() <= tol)     # (|finite values| <= 2)
+            assert same.all(), (out_dtype, act, y[~same][:4], want[~same][:4])
+    y = ops.mxfp4_dense(a, b, act=ops.ACT_RELU)                                                       # no bias
+    assert torch.equal(torch.isnan(y), torch.isnan(z)) and torch.equal(torch.nan_to_num(y), torch.nan_to_num(torch.relu(z)))
