@@ -1088,8 +1088,8 @@ def mxfp4_dequantize(q: Mxfp4, dtype: torch.dtype = torch.float32, out: Optional
 
 
 def mxfp4_from_parts(codes: torch.Tensor, scales: torch.Tensor, cols: int) -> Mxfp4:
-    """an Mxfp4 matrix from packed codes uint8 (rows, 16 * blocks) and one scale byte per block, uint8 (rows, blocks): the
-    scales are laid out once as the kernels read them"""
+    """an Mxfp4 matrix from packed codes uint8 (rows, 16 * blocks) and one scale byte per block, uint8 (rows, blocks): a copy of
+    both, laid out once as the kernels read them"""
     _need(0 < cols <= 1 << 22, "mxfp4_from_parts: columns must be in 1 .. 4194304")
     nb = (int(cols) + 31) // 32
     _dev(codes)
@@ -1098,10 +1098,9 @@ def mxfp4_from_parts(codes: torch.Tensor, scales: torch.Tensor, cols: int) -> Mx
           f"mxfp4_from_parts: scales must be uint8 {(codes.shape[0], nb)} on the codes' device")
     laid = torch.zeros((codes.shape[0], (nb + 15) // 16 * 16), dtype=torch.uint8, device=codes.device)
     laid[:, :nb] = scales
-    codes = codes.contiguous()
+    codes = codes.clone(memory_format=torch.contiguous_format)
     tail = int(cols) % 32
     if tail:                        # codes past the last column are zero
-        codes = codes.clone()
         codes[:, (nb - 1) * 16 + (tail + 1) // 2:] = 0
         if tail % 2:
             codes[:, (nb - 1) * 16 + tail // 2] &= 15

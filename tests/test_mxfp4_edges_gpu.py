@@ -60,3 +60,15 @@ def test_activations_of_infinite_sums(m, n, k, x_four):
             assert same.all(), (out_dtype, act, y[~same][:4], want[~same][:4])
     y = ops.mxfp4_dense(a, b, act=ops.ACT_RELU)                                                       # no bias
     assert torch.equal(torch.isnan(y), torch.isnan(z)) and torch.equal(torch.nan_to_num(y), torch.nan_to_num(torch.relu(z)))
+
+
+@pytest.mark.parametrize("cols", [64, 63, 33])
+def test_from_parts_keeps_a_copy(cols):
+    """the matrix does not follow its parts, whether or not its last block is whole"""
+    from cfd_amd import ops
+    codes = torch.randint(0, 256, (6, 32), dtype=torch.uint8, generator=torch.Generator().manual_seed(1)).cuda()
+    scales = torch.full((6, 2), 127, dtype=torch.uint8, device="cuda")
+    q = ops.mxfp4_from_parts(codes, scales, cols)
+    want = ops.mxfp4_dequantize(q)
+    codes.fill_(0x77), scales.fill_(120)
+    assert torch.equal(ops.mxfp4_dequantize(q), want)
