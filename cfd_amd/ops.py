@@ -1048,6 +1048,18 @@ def _share(a: torch.Tensor, b: torch.Tensor) -> bool:
     return d < wb or d + wa > row
 
 
+def _apart(out: torch.Tensor, *operands: Optional[torch.Tensor]) -> bool:
+    """a matrix with dense rows has no byte in common with any of the dense operands (one may lie between its rows)"""
+    if not out.numel():
+        return True
+    a = out.data_ptr()
+    end = a + ((out.shape[0] - 1) * out.stride(0) + out.shape[1]) * out.element_size()
+    for t in operands:
+        if t is not None and t.data_ptr() < end and a < t.data_ptr() + t.numel() * t.element_size() and _share(out, t.view(1, -1)):
+            return False
+    return True
+
+
 def _mx_quantize(x: torch.Tensor, rows: bool, cols: bool):
     ldx = _mx_input(x, "mxfp4_quantize: x")
     R, K = x.shape
@@ -1082,6 +1094,7 @@ def mxfp4_dequantize(q: Mxfp4, dtype: torch.dtype = torch.float32, out: Optional
         ldy = _mx_input(out, "mxfp4_dequantize: out")
         if not (out.shape == (rows, cols) and out.get_device() == dev):
             _need(False, f"mxfp4_dequantize: out must be {(rows, cols)} on q's device")
+        _need(_apart(out, q.codes, q.scales), "mxfp4_dequantize: out must not overlap q")
         check(_lib.load().cfd_mxfp4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), rows, cols, out.data_ptr(), ldy, _DT[out.dtype],
                                                _raw_stream(dev)), "cfd_mxfp4_dequantize")
     return out
@@ -1113,7 +1126,7 @@ def mxfp4_dense(x: Union[Mxfp4, torch.Tensor], w: Mxfp4, bias: Optional[torch.Te
     4-bit matrix instructions, for training and large batches -- or fp32 / bf16, which keeps the activations' precision and
     reads the weights once (a few rows).  The gradients of y = x w^T are the same product on transposed operands:
     dx = mxfp4_dense(quantize(dy), quantize(w, transpose=True)), dw = mxfp4_dense(quantize(dy, transpose=True),
-    quantize(x, transpose=True))."""
+    quantize(x, transpose=True)).  out: a matrix with dense rows to write into, over none of the operands."""
     lib = _lib.load()
     _mx_check(w, "mxfp4_dense: w")
     n, k = w.shape
@@ -1135,15 +1148,19 @@ def mxfp4_dense(x: Union[Mxfp4, torch.Tensor], w: Mxfp4, bias: Optional[torch.Te
     if odt not in _DT:
         _need(False, f"mxfp4_dense: out_dtype must be fp32 or bf16, is {odt}")
     with _on(dev):
-        if out is None:
+        given = out is not None
+        if not given:
             out = torch.empty((m, n), dtype=odt, device=xt.device)
-        else:
-            if not (out.shape == (m, n) and out.dtype == odt and out.get_device() == dev):
-                _need(False, f"mxfp4_dense: out must be {odt} {(m, n)} on w's device, is {out.dtype} {tuple(out.shape)}")
-            _need(four or not _share(out, x), "mxfp4_dense: out must not overlap x")
+        elif not (out.shape == (m, n) and out.dtype == odt and out.get_device() == dev):
+            _need(False, f"mxfp4_dense: out must be {odt} {(m, n)} on w's device, is {out.dtype} {tuple(out.shape)}")
         if m == 0 or n == 0:
             return out
-        d = Mxfp4DenseDesc(kind, _DT[odt], act, slope, m, n, k, ldx, _mx_input(out, "mxfp4_dense: out"))
+        ldy = _mx_input(out, "mxfp4_dense: out")
+        if given:
+            _need(_apart(out, x.codes, x.scales) if four else not _share(out, x), "mxfp4_dense: out must not overlap x")
+            _need(_apart(out, w.codes, w.scales, bias if bias is None or bias.numel() == n else bias.view(-1)[:n]),
+                  "mxfp4_dense: out must not overlap w or bias")
+        d = Mxfp4DenseDesc(kind, _DT[odt], act, slope, m, n, k, ldx, ldy)
         wsb = lib.cfd_mxfp4_dense_workspace_bytes(m, n, k, kind)
         if wsb < 0:
             check(-1, "cfd_mxfp4_dense_workspace_bytes")

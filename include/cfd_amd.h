@@ -372,7 +372,7 @@ int cfd_mxfp4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t ro
                          void *stream);
 /* y [m][ldy >= n] = act(x w^T + bias), fp32 accumulation.  w: n x k in 4 bits; x: m x k in 4 bits (codes in `x`, x_scales) or
  * float (x [m][ldx >= k], x_scales NULL): then the weights are read once and the activations keep their precision --
- * the form for a few rows.  bias fp32 [n] or NULL; ldy <= 8388608.  ws: cfd_mxfp4_dense_workspace_bytes bytes (may be 0);
+ * the form for a few rows.  bias fp32 [n] or NULL; ldy <= 8388608; y lies over no operand.  ws: cfd_mxfp4_dense_workspace_bytes bytes (may be 0);
  * slices of K are summed in a fixed order: same inputs, same bits. */
 typedef enum { CFD_MX_X_F32 = 0, CFD_MX_X_BF16 = 1, CFD_MX_X_MXFP4 = 2 } cfd_mxfp4_x_kind;
 typedef struct {

@@ -72,3 +72,35 @@ def test_from_parts_keeps_a_copy(cols):
     want = ops.mxfp4_dequantize(q)
     codes.fill_(0x77), scales.fill_(120)
     assert torch.equal(ops.mxfp4_dequantize(q), want)
+
+
+def test_an_output_over_an_operand_is_refused():
+    """a tile would read a bias, codes or scales that another has written; beside them, in one buffer, is allowed"""
+    from cfd_amd import _lib, ops
+    n, k = 24, 40
+    wq, x = ops.mxfp4_quantize(torch.randn(n, k, generator=torch.Generator().manual_seed(1)).cuda()), torch.ones(6, k, device="cuda")
+    buf = torch.zeros(6, 64, device="cuda")
+    bias = torch.arange(float(n), device="cuda")
+    out = buf[:, :n]
+    for a in (x, ops.mxfp4_quantize(x)):
+        for over in (buf[2, :n], buf[5, 20:44], buf[0, n - 1:2 * n - 1], buf.view(-1)):
+            with pytest.raises(_lib.CfdError):
+                ops.mxfp4_dense(a, wq, bias=over, out=out)
+        assert not buf.any()
+        buf[3, n:2 * n] = bias
+        assert torch.equal(ops.mxfp4_dense(a, wq, bias=buf[3, n:2 * n], out=out), ops.mxfp4_dense(a, wq, bias=bias))
+        buf.zero_()
+    # a 4-bit matrix inside the output's bytes: its codes or its scales alone, on either side and in the decoding
+    room = torch.zeros(64 * 64, device="cuda").view(torch.uint8)
+    q = ops.mxfp4_quantize(torch.ones(n, k, device="cuda"))
+    for name in ("codes", "scales"):
+        part = getattr(q, name)
+        inside = room[:part.numel()].view(part.shape)
+        inside.copy_(part)
+        over = q._replace(**{name: inside})
+        y = room.view(torch.float32)
+        for call in (lambda: ops.mxfp4_dense(x, over, out=y[:6 * n].view(6, n)), lambda: ops.mxfp4_dense(over, over, out=y[:n * n].view(n, n)),
+                     lambda: ops.mxfp4_dense(over, q, out=y[:n * n].view(n, n)), lambda: ops.mxfp4_dequantize(over, out=y[:n * k].view(n, k))):
+            with pytest.raises(_lib.CfdError):
+                call()
+        assert torch.equal(inside, part)

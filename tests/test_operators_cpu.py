@@ -153,3 +153,18 @@ def test_mxfp4_plan_reaches_every_way_of_sharing(lib):
     assert {(rows, slices > 1) for rows, slices, *_ in four} == {(r, s) for r in (64, 256) for s in (True, False)}
     assert lib.cfd_mxfp4_dense_plan(4, 4, 0, 2, None) < 0 and lib.cfd_mxfp4_dense_plan(4, 4, 64, 3, (C.c_int * 4)()) < 0
     _refused(lib, lib.cfd_mxfp4_dense_plan(0, 4, 64, 2, (C.c_int * 4)()), "bad arguments")
+
+
+def test_an_output_over_an_operand_is_seen():
+    """_apart on views of one buffer: between the rows of an output or behind it is beside it, one byte inside is over it"""
+    from cfd_amd import ops
+    buf = torch.zeros(6, 64)
+    flat, raw = buf.view(-1), buf.view(-1).view(torch.uint8)
+    out = buf[:, :24]
+    assert ops._apart(out, None, buf[2, 24:48], flat[24:64], flat[5 * 64 + 24:], torch.zeros(24), raw[96:256].view(10, 16))
+    for t in (buf[2, 23:47], buf[2, 40:].contiguous().set_(flat[150:220]), flat[:1], flat[5 * 64 + 23:], flat[60:65], raw[95:111], raw[96:257], buf):
+        assert not ops._apart(out, None, t), t.shape
+    assert ops._apart(buf[:1, :24], flat[24:]) and not ops._apart(buf[:1, :24], flat[23:])
+    assert ops._apart(buf[:0], buf) and ops._apart(buf[:, :0], buf)
+    half = torch.zeros(4, 10, dtype=torch.bfloat16)
+    assert not ops._apart(half[:, :3], half.view(-1)[32:33]) and ops._apart(half[:, :3], half.view(-1)[33:40])
