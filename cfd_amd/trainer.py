@@ -69,8 +69,9 @@ class AdamW:
 
     params: dense fp32 or bf16 tensors of one dtype, updated in place; copies: bf16 tensors of the same lengths that receive
     fp32 parameters as the matrix kernels read them (None: none); weight_decay: one value or one per tensor (0 for
-    biases and BatchNorm, as Keras' exclude_from_weight_decay).  lr is read at every step; an fp32 device tensor of one
-    element may be given instead, for a schedule inside a captured graph.
+    biases and BatchNorm, as Keras' exclude_from_weight_decay).  lr, b1, b2, eps, weight_decay and seed may be assigned: the next
+    step uses them (a captured step keeps what it was captured with).  For lr an fp32 device tensor of one element may be given,
+    for a schedule inside a captured graph.
 
     State, flat over all tensors (segment i at offsets[i], padded to 256 with zeros), for checkpoints and inspection:
     m, v (fp32, or float8_e4m3fn / float8_e5m2 codes with m_scale, v_scale fp32: value = code * scale[element // 256]) and
@@ -87,9 +88,8 @@ class AdamW:
         ops._tensor_list(self.params, "AdamW: parameters")
         p0 = self.params[0]
         self.device = p0.device
-        self.weight_decay = [float(weight_decay)] * n if isinstance(weight_decay, (int, float)) else [float(d) for d in weight_decay]
-        if len(self.weight_decay) != n:
-            raise ValueError(f"AdamW: {len(self.weight_decay)} weight decays for {n} parameters")
+        self._table, self._desc = (ops.AdamwTensor * n)(), ops.AdamwDesc(p_dtype=ops._DT[p0.dtype], state_bits=state_bits)
+        self.weight_decay = weight_decay
         if self.copies is not None:
             if p0.dtype != torch.float32 or len(self.copies) != n:
                 raise ValueError("AdamW: copies need fp32 parameters, one each")
@@ -98,14 +98,13 @@ class AdamW:
                 raise ValueError("AdamW: a copy must have its parameter's length")
         if state_bits not in (8, 32):
             raise ValueError("AdamW: state_bits must be 8 or 32")
-        if not (0.0 <= beta_1 < 1.0 and 0.0 <= beta_2 < 1.0 and epsilon >= 1e-12):
-            raise ValueError("AdamW: beta must be in [0, 1) and epsilon at least 1e-12")
         if isinstance(lr, torch.Tensor):
             self._need_scalar(lr, "AdamW: a learning-rate tensor")
         spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in self.params + (self.copies or []) if t.numel())
         if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
             raise ValueError("AdamW: parameters (and copies) must not overlap")
-        self.lr, self.b1, self.b2, self.eps, self.state_bits, self.seed = lr, beta_1, beta_2, epsilon, state_bits, int(seed)
+        self.state_bits = state_bits
+        self.lr, self.b1, self.b2, self.eps, self.seed = lr, beta_1, beta_2, epsilon, seed
         self.offsets, off = [], 0
         for p in self.params:
             self.offsets.append(off)
@@ -119,16 +118,70 @@ class AdamW:
             self.m_scale, self.v_scale = z(off // ops.ADAMW_BLOCK, torch.float32), z(off // ops.ADAMW_BLOCK, torch.float32)
         self.t = z(1, torch.int32)
         self._ws = z(32, torch.uint8)
-        self._table = (ops.AdamwTensor * n)()
-        self._desc = ops.AdamwDesc(p_dtype=ops._DT[p0.dtype], state_bits=state_bits, seed=self.seed & 0xffffffff, eps=epsilon,
-                                   beta1=beta_1, beta2=beta_2)
         self._sizes = [p.numel() for p in self.params]
         self._grad_column = np.frombuffer(self._table, dtype=np.int64)[ops.AdamwTensor.g.offset // 8::ops.C.sizeof(ops.AdamwTensor) // 8]
         for k, p in enumerate(self.params):
             e = self._table[k]
-            e.p, e.n, e.state_offset, e.weight_decay = p.data_ptr(), p.numel(), self.offsets[k], self.weight_decay[k]
+            e.p, e.n, e.state_offset = p.data_ptr(), p.numel(), self.offsets[k]
             e.copy = self.copies[k].data_ptr() if self.copies is not None else None
         self._ptrs = self._addresses()
+
+    # hyper-parameters live in the records that every step hands to the kernels
+    @staticmethod
+    def _beta(x) -> float:
+        if not 0.0 <= x < 1.0:
+            raise ValueError(f"AdamW: beta must be in [0, 1), is {x}")
+        return float(x)
+
+    @property
+    def b1(self) -> float:
+        return self._desc.beta1
+
+    @b1.setter
+    def b1(self, x) -> None:
+        self._desc.beta1 = self._beta(x)
+
+    @property
+    def b2(self) -> float:
+        return self._desc.beta2
+
+    @b2.setter
+    def b2(self, x) -> None:
+        self._desc.beta2 = self._beta(x)
+
+    @property
+    def eps(self) -> float:
+        return self._eps
+
+    @eps.setter
+    def eps(self, x) -> None:
+        if not x >= 1e-12:
+            raise ValueError(f"AdamW: epsilon must be at least 1e-12, is {x}")
+        self._eps = self._desc.eps = float(x)
+
+    @property
+    def seed(self) -> int:
+        return self._seed
+
+    @seed.setter
+    def seed(self, x) -> None:
+        self._seed = int(x)
+        self._desc.seed = self._seed & 0xffffffff
+
+    @property
+    def weight_decay(self):
+        """one value per tensor; assigned as a whole, from one value or one per tensor"""
+        return self._weight_decay
+
+    @weight_decay.setter
+    def weight_decay(self, x) -> None:
+        n = len(self._table)
+        each = (float(x),) * n if isinstance(x, (int, float)) else tuple(float(d) for d in x)
+        if len(each) != n:
+            raise ValueError(f"AdamW: {len(each)} weight decays for {n} parameters")
+        self._weight_decay = each
+        for e, d in zip(self._table, each):
+            e.weight_decay = d
 
     def _addresses(self):
         state = [self.m, self.v, self.t] + ([self.m_scale, self.v_scale] if self.state_bits == 8 else [])
