@@ -65,7 +65,8 @@ class Adam:
 class AdamW:
     """keras.optimizers.AdamW(learning_rate, weight_decay, beta_1, beta_2, epsilon) over a list of tensors, one launch per
     64 of them, with the state in fp32 (state_bits=32) or in 8 bits with a power-of-two scale per 256 elements (state_bits=8:
-    16 instead of 28 bytes of traffic per fp32 parameter, 2 instead of 8 bytes of state; cfd_adamw_step has the formulas).
+    16 instead of 28 bytes of traffic per fp32 parameter, 2 instead of 8 bytes of state; cfd_adamw_step has the formulas and what its
+    rounding loses; beta_1 and beta_2 are at most 0.9999 then).
 
     params: dense fp32 or bf16 tensors of one dtype, updated in place; copies: bf16 tensors of the same lengths that receive
     fp32 parameters as the matrix kernels read them (None: none); weight_decay: one value or one per tensor (0 for
@@ -127,10 +128,9 @@ class AdamW:
         self._ptrs = self._addresses()
 
     # hyper-parameters live in the records that every step hands to the kernels
-    @staticmethod
-    def _beta(x) -> float:
-        if not 0.0 <= x < 1.0:
-            raise ValueError(f"AdamW: beta must be in [0, 1), is {x}")
+    def _beta(self, x) -> float:
+        if not (0.0 <= x < 1.0 and (self.state_bits == 32 or x <= 0.9999)):
+            raise ValueError(f"AdamW: beta must be in [0, 1), with an 8-bit state at most 0.9999, is {x}")
         return float(x)
 
     @property

@@ -168,3 +168,29 @@ def test_an_output_over_an_operand_is_seen():
     assert ops._apart(buf[:0], buf) and ops._apart(buf[:, :0], buf)
     half = torch.zeros(4, 10, dtype=torch.bfloat16)
     assert not ops._apart(half[:, :3], half.view(-1)[32:33]) and ops._apart(half[:, :3], half.view(-1)[33:40])
+
+
+def test_what_stochastic_rounding_cuts():
+    """over all 65536 draws a stored value is low by 0 to 2^-16 of its code's spacing in the mean, never high"""
+    x = np.abs(np.random.default_rng(1).standard_normal(256)) * 10.0 ** np.random.default_rng(2).uniform(-3, 0, 256)
+    for enc in (OO.encode_m, OO.encode_v):
+        lo, s = enc(x, np.zeros(256))
+        hi, _ = enc(x, np.full(256, 65535.0))
+        total = np.zeros(256)
+        for u in range(0, 65536, 4096):
+            q, _ = enc(np.tile(x, 4096), np.repeat(np.arange(u, u + 4096.0), 256))
+            total += q.reshape(4096, 256).sum(0)
+        low = (x - total / 65536 * s) / ((hi - lo) * s)
+        assert (hi > lo).all() and low.min() >= -1e-9 and low.max() <= 2.0 ** -16
+
+
+def test_adamw_refuses_a_slow_beta_in_8_bits(lib):
+    """past 0.9999 what an 8-bit state's rounding cuts is no longer small beside a step's movement"""
+    from cfd_amd._lib import AdamwDesc, AdamwTensor
+    t = (AdamwTensor * 1)()
+    t[0].p = t[0].g = 1 << 20
+    t[0].n = 10
+    good = dict(p_dtype=0, g_dtype=0, state_bits=8, seed=0, lr=1e-3, eps=1e-7, beta1=0.9, beta2=0.999)
+    for kw in (dict(beta1=0.99991), dict(beta2=0.99999)):
+        d = AdamwDesc(**{**good, **kw})
+        _refused(lib, lib.cfd_adamw_step(t, 1, C.byref(d), P, P, P, P, P, None, None, P, None), "0.9999")

@@ -35,3 +35,34 @@ def test_attributes_take_effect_at_the_next_step(bits):
     with pytest.raises(TypeError):
         opt.weight_decay[0] = 0.5
     _check_step(opt, _views(sizes, torch.float32, 17), None, lr, wd)
+
+
+@pytest.mark.parametrize("beta_2", [0.999, 0.9999])
+def test_what_the_8_bit_state_settles_at(beta_2):
+    """v of a constant gradient after four times 1 / (1 - beta_2) steps.  Each step stores it low by 0 to 2^-16 spacings of a quarter at
+    most, 2^-18 of the value: 2^-18 / (1 - beta_2) in all.  The recursion's four fp32 roundings a step, 2^-24 each, add
+    2^-22 / (1 - beta_2) either way; the mean of n elements has a standard error."""
+    from cfd_amd import trainer
+    n, steps = 1 << 18, int(4 / (1 - beta_2))
+    g = torch.full((n,), 1.3, device="cuda").sqrt()
+    opt = trainer.AdamW([torch.zeros(n, device="cuda")], lr=0.0, beta_2=beta_2, weight_decay=0.0, state_bits=8, seed=11)
+    for _ in range(steps):
+        opt.step([g])
+    v = (opt.v.float() * opt.v_scale.repeat_interleave(256)).double()
+    want = 1.3 * (1 - beta_2 ** steps)
+    off, noise = (float(v.mean()) - want) / want, 5 * float(v.std()) / n ** 0.5 / want + 2.0 ** -22 / (1 - beta_2)
+    print(f"beta_2 {beta_2}: v {100 * off:.3f} %, 5 standard errors and fp32 {100 * noise:.3f} %")
+    assert -(2.0 ** -18 / (1 - beta_2)) - noise <= off <= noise
+
+
+def test_slow_betas_need_a_32_bit_state():
+    from cfd_amd import trainer
+    p = torch.zeros(8, device="cuda")
+    opt = trainer.AdamW([p], beta_1=0.9999, beta_2=0.9999, state_bits=8)
+    for kw in (dict(beta_1=0.99991), dict(beta_2=0.99999)):
+        with pytest.raises(ValueError):
+            trainer.AdamW([p], state_bits=8, **kw)
+        trainer.AdamW([p], **kw).step([torch.ones_like(p)])
+    with pytest.raises(ValueError):
+        opt.b2 = 0.99999
+    opt.step([torch.ones_like(p)])
