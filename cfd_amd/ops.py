@@ -950,7 +950,8 @@ def _tensor_list(ts: Sequence[torch.Tensor], what: str, dtype: Optional[torch.dt
 
 def grad_norm(grads: Union[torch.Tensor, Sequence[torch.Tensor]], max_norm: float, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """fp32 device tensor [norm, scale]: the L2 norm over all elements of `grads` (dense tensors of one dtype, any length) and
-    min(1, max_norm / norm), NaN where the norm is not finite.  Nothing waits for the device: hand out[1:] to
+    min(1, max_norm / norm), NaN where the norm is not finite (fp64: one past fp32's range reads as infinity, its scale is still the
+    quotient).  Nothing waits for the device: hand out[1:] to
     trainer.AdamW.step as `grad_scale` and the step is clipped, or skipped on a non-finite gradient."""
     lib = _lib.load()
     grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
@@ -1124,7 +1125,7 @@ def mxfp4_dense(x: Union[Mxfp4, torch.Tensor], w: Mxfp4, bias: Optional[torch.Te
                 out_dtype: Optional[torch.dtype] = None, out: Optional[torch.Tensor] = None, slope: float = LEAKY_SLOPE) -> torch.Tensor:
     """y (m, n) = act(x w^T + bias), fp32 accumulation.  w: (n, k) in 4 bits.  x: (m, k) in 4 bits -- both operands on the
     4-bit matrix instructions, for training and large batches -- or fp32 / bf16, which keeps the activations' precision and
-    reads the weights once (a few rows).  The gradients of y = x w^T are the same product on transposed operands:
+    reads the weights once for every 48 bf16 or 16 fp32 rows (the form for a few rows).  The gradients of y = x w^T are the same product on transposed operands:
     dx = mxfp4_dense(quantize(dy), quantize(w, transpose=True)), dw = mxfp4_dense(quantize(dy, transpose=True),
     quantize(x, transpose=True)).  out: a matrix with dense rows to write into, over none of the operands."""
     lib = _lib.load()

@@ -192,7 +192,7 @@ class AdamW:
             raise ValueError(f"{what} must be one fp32 element on the parameters' device")
 
     def step(self, grads, grad_scale=None) -> None:
-        """One update from `grads` (one dense fp32 or bf16 tensor per parameter, one dtype).  grad_scale: None, or an fp32
+        """One update from `grads` (one dense fp32 or bf16 tensor per parameter, one dtype, apart from parameters and state).  grad_scale: None, or an fp32
         device tensor of one element that multiplies every gradient (ops.grad_norm(...)[1:]); where it is not finite the
         whole step is skipped, t included."""
         grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)

@@ -320,7 +320,8 @@ int cfd_adam_step(float *w, const float *g, float *m, float *v, void *w_compute,
  *
  * Global L2 norm of `count` gradients g[i] of n[i] elements (n[i] may be 0; one dtype for all, any alignment) and the factor
  * that clips it: out[0] = norm, out[1] = min(1, max_norm / norm), or NaN where the norm is not finite.  Squares and
- * sums in fp64, in a fixed order.  ws: cfd_grad_norm_workspace_bytes(n, count) bytes, 8-byte aligned. */
+ * sums in fp64, in a fixed order (a norm past fp32's range reads as infinity, its factor is still the quotient).
+ * ws: cfd_grad_norm_workspace_bytes(n, count) bytes, 8-byte aligned. */
 int64_t cfd_grad_norm_workspace_bytes(const int64_t *n, int count);
 int cfd_grad_norm(const void *const *g, const int64_t *n, int count, int dtype, float max_norm, void *ws, float *out,
                   void *stream);
@@ -334,10 +335,11 @@ int cfd_grad_norm(const void *const *g, const int64_t *n, int count, int dtype, 
  *   state_bits 32: m, v fp32 [state elements]; m_scale, v_scale unused.
  *   state_bits  8: m e4m3 codes, v e5m2 codes [state elements], m_scale, v_scale fp32 [state elements / 256]: the value
  *     is code * scale[element / 256].  Stored by stochastic rounding from a hash of (seed, t, position), 16 bits a
- *     draw: the expected state is the 32-bit recursion's, its magnitudes low by 2^-16 / (1 - beta) of a code's spacing at most (v: 0.4 % at
- *     beta2 = 0.999, 3.8 % at 0.9999; beta1, beta2 <= 0.9999 here); v > 0 never rounds to 0.  A block of 256 with an infinity or NaN gets a NaN scale.
- * Tensor i's state starts at state_offset (a multiple of 256; its segment is padded to one with zeros).  Tensors and
- * their state segments must not overlap. */
+ *     draw: the expected state is the 32-bit recursion's, its magnitudes low by 2^-16 / (1 - beta) of a code's spacing
+ *     at most (v: 0.4 % at beta2 = 0.999, 3.8 % at 0.9999; beta1, beta2 <= 0.9999 here); v > 0 never rounds to 0.  A block
+ *     of 256 with an infinity or NaN gets a NaN scale.
+ * Tensor i's state starts at state_offset (a multiple of 256; its segment is padded to one with zeros).  Tensors,
+ * copies, state segments and the device scalars must not overlap each other or the gradients. */
 typedef struct {
   void *p;             /* p_dtype [n] */
   const void *g;       /* g_dtype [n] */
@@ -372,9 +374,9 @@ int cfd_mxfp4_quantize(const void *x, int64_t ldx, int dtype, int64_t rows, int6
 int cfd_mxfp4_dequantize(const uint8_t *codes, const uint8_t *scales, int64_t rows, int64_t cols, void *y, int64_t ldy, int dtype,
                          void *stream);
 /* y [m][ldy >= n] = act(x w^T + bias), fp32 accumulation.  w: n x k in 4 bits; x: m x k in 4 bits (codes in `x`, x_scales) or
- * float (x [m][ldx >= k], x_scales NULL): then the weights are read once and the activations keep their precision --
- * the form for a few rows.  bias fp32 [n] or NULL; ldy <= 8388608; y lies over no operand.  ws: cfd_mxfp4_dense_workspace_bytes bytes (may be 0);
- * slices of K are summed in a fixed order: same inputs, same bits. */
+ * float (x [m][ldx >= k], x_scales NULL): then the activations keep their precision and the weights are read once for
+ * every 48 bf16 or 16 fp32 rows -- the form for a few rows.  bias fp32 [n] or NULL; ldy <= 8388608; y lies over no operand.
+ * ws: cfd_mxfp4_dense_workspace_bytes bytes (may be 0); slices of K are summed in a fixed order: same inputs, same bits. */
 typedef enum { CFD_MX_X_F32 = 0, CFD_MX_X_BF16 = 1, CFD_MX_X_MXFP4 = 2 } cfd_mxfp4_x_kind;
 typedef struct {
   int x_kind, out_dtype, act;

@@ -66,3 +66,10 @@ def test_slow_betas_need_a_32_bit_state():
     with pytest.raises(ValueError):
         opt.b2 = 0.99999
     opt.step([torch.ones_like(p)])
+
+
+def test_a_norm_past_fp32_reads_as_infinity_and_still_clips():
+    """the factor is the fp64 quotient rounded once: half of fp32's smallest subnormal"""
+    from cfd_amd import ops
+    n = ops.grad_norm([torch.full((100,), 3e38, device="cuda")], 1.0)
+    assert float(n[0]) == float("inf") and abs(float(n[1]) - 1 / (10 * float(torch.tensor(3e38)))) <= 2.0 ** -150
