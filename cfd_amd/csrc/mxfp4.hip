@@ -17,7 +17,6 @@ typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4a4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef __bf16 bf16x8a2 __attribute__((ext_vector_type(8), aligned(2)));
-typedef __bf16 bf16x4a2 __attribute__((ext_vector_type(4), aligned(2)));
 
 // threads of a launch per matrix row: a 64-bit division by it would be most of a streaming kernel's instructions
 struct FastDiv {
@@ -919,8 +918,9 @@ static void mx_plan(MxDense &p, int x_kind) {
     const int most = x_kind == CFD_MX_X_BF16 ? 48 : 16;
     p.mt = (p.M + most - 1) / most;
     p.xrows = (p.M + p.mt - 1) / p.mt;
-    // Four waves on one weight tile where each has one K group, or its few columns are cheap to convert four times as often: a
-    // wave's loads of 16 rows at a time keep a CU's address unit busy, and so they spread over more CUs.  Us, four waves on a tile | four
+    // Four waves on one weight tile where the chip has room for a workgroup per tile and K group (two on each of 256 CUs: a slice is then one
+    // group, all four waves convert it and one multiplies), or where few columns are cheap to convert four times as often: a wave's
+    // loads of 16 rows at a time keep a CU's address unit busy, and so they spread over more CUs.  Us, four waves on a tile | four
     // tiles: 1 row fp32 256 x 2048 7.1 | 9.0, 256 x 262144 14.0 | 16.9, 28672 x 8192 27.2 | 36.0; 16 rows bf16 4096^2 11.1 | 12.3, 8192^2
     // 19.8 | 19.3, 28672 x 8192 50 | 42; 48 rows bf16 256 x 2048 13.0 | 17.8, 256 x 65536 18.9 | 21.7, 1030 x 16384 31 | 20
     const int groups = (p.nb + 15) / 16, cols = (x_kind == CFD_MX_X_BF16 ? 1 : 3) * p.xrows;

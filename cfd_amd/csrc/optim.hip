@@ -62,7 +62,7 @@ template <typename T> __device__ __forceinline__ void store4(T *p, int left, con
   }
 }
 
-__host__ __device__ __forceinline__ unsigned hash32(unsigned x) {   // a 32-bit bijection with full avalanche
+__host__ __device__ __forceinline__ unsigned hash32(unsigned x) {   // a bijection; shifts and factors: C. Wellons (2018), found by search for the least avalanche bias
   x ^= x >> 16; x *= 0x7feb352du;
   x ^= x >> 15; x *= 0x846ca68bu;
   return x ^ (x >> 16);
