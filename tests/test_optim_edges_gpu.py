@@ -73,3 +73,41 @@ def test_a_norm_past_fp32_reads_as_infinity_and_still_clips():
     from cfd_amd import ops
     n = ops.grad_norm([torch.full((100,), 3e38, device="cuda")], 1.0)
     assert float(n[0]) == float("inf") and abs(float(n[1]) - 1 / (10 * float(torch.tensor(3e38)))) <= 2.0 ** -150
+
+
+def test_flat_ranges_of_a_parameter_store_step_like_its_tensors():
+    """neighbours of one decay as one tensor, their zero padding between them: parameters, copies and norm are those of the list of views"""
+    from cfd_amd import nets, ops, trainer
+    got = []
+    for flat in (False, True):
+        net = nets.CnnRegressor((16, 64, 1), dtype=torch.bfloat16, seed=5)
+        P = net.params
+        P.enable_training()
+        P.grad.copy_(torch.randn(P.n_trainable, generator=torch.Generator().manual_seed(3)))
+        names, spans = [], []
+        for name, s in sorted(P.specs.items(), key=lambda kv: kv[1].offset):
+            if s.kind != "stat":
+                decay = 0.004 if name.endswith("kernel") else 0.0
+                spans = spans if spans and spans[-1][1] == decay else spans + [(s.offset, decay)]
+                names.append((name, decay))
+        cuts = [a for a, _ in spans] + [P.n_trainable]
+        ranges = [slice(a, b) for a, b in zip(cuts, cuts[1:])]
+        live = torch.zeros_like(P.grad)
+        for name, _ in names:
+            o, n = P.specs[name].offset, P.specs[name].numel
+            live[o:o + n] = 1
+        P.grad.mul_(live)
+        assert not (P.master[:P.n_trainable] * (1 - live)).any() and len(ranges) < len(names)
+        if flat:
+            opt = trainer.AdamW([P.master[r] for r in ranges], copies=[P.compute[r] for r in ranges], weight_decay=[d for _, d in spans], **HYPER)
+            grads = [P.grad[r] for r in ranges]
+        else:
+            opt = trainer.AdamW([P.m(n) for n, _ in names], copies=[P.c(n) for n, _ in names], weight_decay=[d for _, d in names], **HYPER)
+            grads = [P.g(n) for n, _ in names]
+        norms = [ops.grad_norm(P.grad if flat else grads, 0.1) for _ in range(3)]
+        for n in norms:
+            opt.step(grads, torch.full((1,), 0.01, device="cuda"))
+        got.append((P.master.clone(), P.compute.clone(), norms[0]))
+    (a, ca, na), (b, cb, nb) = got
+    assert torch.equal(a, b) and torch.equal(ca, cb)
+    assert (na - nb).abs().max() <= 2.0 ** -23 * na.abs().max()     # (fp64 sums in another order, rounded once)
