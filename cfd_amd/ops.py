@@ -1090,12 +1090,14 @@ def mxfp4_dequantize(q: Mxfp4, dtype: torch.dtype = torch.float32, out: Optional
     _mx_check(q, "mxfp4_dequantize: q")
     (rows, cols), dev = q.shape, q.codes.get_device()
     with _on(dev):
-        if out is None:
+        given = out is not None
+        if not given:
             out = torch.empty((rows, cols), dtype=dtype, device=q.codes.device)
         ldy = _mx_input(out, "mxfp4_dequantize: out")
         if not (out.shape == (rows, cols) and out.get_device() == dev):
             _need(False, f"mxfp4_dequantize: out must be {(rows, cols)} on q's device")
-        _need(_apart(out, q.codes, q.scales), "mxfp4_dequantize: out must not overlap q")
+        if given:
+            _need(_apart(out, q.codes, q.scales), "mxfp4_dequantize: out must not overlap q")
         check(_lib.load().cfd_mxfp4_dequantize(q.codes.data_ptr(), q.scales.data_ptr(), rows, cols, out.data_ptr(), ldy, _DT[out.dtype],
                                                _raw_stream(dev)), "cfd_mxfp4_dequantize")
     return out
