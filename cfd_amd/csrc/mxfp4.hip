@@ -328,8 +328,10 @@ struct MxDense {
 
 // activation of a sum.  ReLU by comparison, not by a slope of zero: a sum of -infinity is 0 (its product with zero would be NaN), and NaN stays
 __device__ __forceinline__ float mx_relu(float v) { return v < 0.f ? 0.f : v; }
-__device__ __forceinline__ float mx_act(const MxDense &p, float v) {
-  return p.act == CFD_ACT_RELU ? mx_relu(v) : apply_act(v, p.act, p.slope);
+__device__ __forceinline__ float mx_act(const MxDense &p, float v) {   // (without a branch between the linear kinds)
+  if (p.act == CFD_ACT_SIGMOID) return 1.f / (1.f + __expf(-v));
+  const float ns = act_neg_scale(p.act, p.slope), lo = p.act == CFD_ACT_RELU ? 0.f : -INFINITY;
+  return v < 0.f ? fmaxf(v, lo) * ns : v;
 }
 __device__ __forceinline__ void mx_store(const MxDense &p, int64_t m, int n, float v) {   // one element of the output
   if (p.out_bf16) ((bf16 *)p.y)[m * p.ldy + n] = (bf16)v;
