@@ -153,7 +153,7 @@ __device__ __forceinline__ unsigned quad_bytes(unsigned byte) {   // the same ov
 }
 
 // rows only: four lanes share a block of 32 (eight columns each): 32-byte / 16-byte loads, 4-byte stores, the block's
-// maximum in two DPP steps.  HBM-bound, 2 (bf16) or 4 bytes in and 0.53 out an element: 64 x 262144 bf16 (42.5 MB) take 8.9 us,
+// maximum in two DPP steps.  HBM-bound, 2 (bf16) or 4 bytes in and 0.53 out an element: 64 x 262144 bf16 (42.5 MB) take 8.8 us,
 // 4.8 TB/s.  A row is walked in multiples of 128 columns, so that 16 lanes hold four whole scale bytes.
 template <typename T> __global__ __launch_bounds__(256) void mx_quant_rows_kernel(const T *x, int64_t ldx, int64_t rows, int K,
                                                                                    int nb, int pitch, uint8_t *codes,
@@ -173,7 +173,7 @@ template <typename T> __global__ __launch_bounds__(256) void mx_quant_rows_kerne
 // both orientations from one read: a 128 x 128 tile; rows are coded on the way in, columns from LDS, two adjacent columns and 32
 // rows a thread.  LDS words are swizzled by 16 per 32 rows: the four row blocks that a quad of lanes reads lie in different banks.
 // Codes leave as 64 contiguous bytes a row in both orientations.  Near a copy's rate where there are tiles for several rounds (8192 x 4096
-// fp32, 170 MB: 35 us, 4.9 TB/s); one round fills and drains the chip in ~4 us beside the bytes' time (4090 x 4102, 85 MB: 22.2 us).
+// fp32, 170 MB: 33 us, 5.1 TB/s); one round fills and drains the chip in ~4 us beside the bytes' time (4090 x 4102, 85 MB: 22.1 us).
 constexpr int QT = 128;
 template <typename T> __global__ __launch_bounds__(256) void mx_quant_both_kernel(const T *x, int64_t ldx, int R, int K,
                                                                                    int nb, int pitch, uint8_t *codes,
@@ -274,7 +274,7 @@ __device__ __forceinline__ bf16x8 mx_bf16x8(unsigned c, float s) {     // eight 
 __device__ __forceinline__ float mx_scale_or_nan(unsigned byte) { return byte == 255u ? __uint_as_float(0x7fc00000u) : mx_scale_f32(byte); }
 
 // codes -> values (exact, or an overflow to infinity at the top of the scale's range): a lane reads eight codes and writes 16 (bf16)
-// or 32 (fp32) bytes.  HBM-bound: 64 x 262144 to bf16 (42.5 MB) 8.7 us, 4.9 TB/s.
+// or 32 (fp32) bytes.  HBM-bound: 64 x 262144 to bf16 (42.5 MB) 8.8 us, 4.8 TB/s.
 template <typename T> __global__ __launch_bounds__(256) void mx_dequant_kernel(const uint8_t *codes, const uint8_t *scales,
                                                                                 int64_t rows, int K, int nb, int pitch, T *y,
                                                                                 int64_t ldy, FastDiv G) {
@@ -426,8 +426,8 @@ __device__ __forceinline__ void mx_wait_lds() { asm volatile("s_waitcnt lgkmcnt(
 // of each operand) in two stages, the 16 scale bytes a row of a group in two more; the next half is under way while this one
 // multiplies.  16x16x128 scaled MFMA: lane = row l & 15, step s takes block 4s + (l >> 4), a lane shifts its scale byte down.
 // Chunks are XOR-ed with bits 1-3 of the row (see the 256 x 256 kernel).  Codes behind the last column (the next row's) need no
-// mask: their scale bytes are zero on both operands, 2^-254 is zero in fp32.  128 x 262144 x 256 (53.5 MB): 16.8 us, 3.2 TB/s; its 32 slices
-// are summed in 3.9 us more.
+// mask: their scale bytes are zero on both operands, 2^-254 is zero in fp32.  128 x 262144 x 256 (53.5 MB): 16.7 us, 3.2 TB/s; its 32 slices
+// are summed in 3.9 us more.  A K of 512 columns or fewer is one group and one wave's: 64 x 256 x 262144 to bf16 (69 MB) takes 90 us.
 constexpr int MXD_OPER = 64 * 128, MXD_STAGE = 2 * MXD_OPER, MXD_WAVE = 2 * MXD_STAGE + 2 * 2048, MXD_LDS = 4 * MXD_WAVE;   // 144 KiB
 __global__ __launch_bounds__(256, 1) void mx_dense_kernel(MxDense p) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -533,7 +533,7 @@ __global__ __launch_bounds__(256, 1) void mx_dense_kernel(MxDense p) {
 //     load every four MFMAs (in bursts of eight: 3 % slower at 4096 x 4096 x 8192).
 // The K range goes in groups of two K tiles; codes behind the last column need no mask: their scale bytes are zero on both
 // operands, and 2^-254 is zero in fp32.  Reads past the operand are cut off by the buffer's size, which shrinks as its base advances.
-// 4096 x 8192 x 4096 takes 65 us, 4.2 PFLOP/s; the same MFMAs on registers alone run at 6.65.
+// 4096 x 8192 x 4096 takes 64-67 us, 4.1-4.3 PFLOP/s; the same MFMAs on registers alone run at 6.65.
 constexpr int MXT_OPER = 256 * 128, MXT_SCALE = 4 * MXT_OPER, MXT_SCALE_STAGE = 512 * 16;   // W0, W1, X0, X1, scales
 constexpr int MXT_LDS = MXT_SCALE + 2 * MXT_SCALE_STAGE;   // 144 KiB
 
@@ -779,8 +779,8 @@ template <typename TO, int MODE> __global__ __launch_bounds__(256, 1) void mx_de
 // the activations in 16x16x32 bf16 MFMAs, whose k order is the lane's block order on both operands.  The activations of a K
 // group are converted once per workgroup and wait in LDS as columns of the product: up to 48 rows in bf16, or 16 in fp32, which
 // are split exactly into three bf16 terms (8 + 8 + 8 bits by truncation), a column each -- fp32 accuracy, and one row costs one
-// MFMA, not three.  A row's three columns are added when the waves join.  One fp32 row on 262144 x 256 (36 MB): 10.8 us, the latency of one round
-// of loads on top of 3.3 TB/s; the slices' sum takes 3.8 more.
+// MFMA, not three.  A row's three columns are added when the waves join.  One fp32 row on 262144 x 256 (36 MB): 10.5 us, the latency of one round
+// of loads on top of 3.3 TB/s; the slices' sum takes 2.6-3.9 more.
 struct Split3 { bf16 t[3]; };
 __device__ __forceinline__ Split3 split3(float x) {
   Split3 r;
